@@ -1,0 +1,213 @@
+// Block tables, row offsets, positions and slots of a serving step from the requests' lengths.
+//
+// Three prefix sums over the requests in order - rows, pages taken, pages given back - say everything: a request is admitted
+// while its inclusive sums fit the rows and the free pages, both of which only grow, so the refused requests with rows are a
+// tail and the offsets are the sums cut off at the last admitted one.  Row r then belongs to the last request whose offset is
+// at most r, found by bisection in shared memory; the same for the pages.
+//
+// What bounds it: latency (a few kilobytes in, 8 bytes per row out).  So it is one launch: a cluster of eight blocks, every one
+// of which reads the requests and sums them by itself, waits until all have read (the outputs may be the inputs), and writes
+// its share.  A step of a few rows takes one block.
+#include <cooperative_groups.h>
+
+#include "serve.cuh"
+
+namespace b200 {
+
+constexpr int PP_THREADS = 512;
+constexpr int PP_EACH = 4;                       // requests of a thread
+constexpr int PP_BATCH = PP_THREADS * PP_EACH;
+
+struct PlanArgs {
+    const int32_t *ctx, *fresh, *held;
+    int batch;
+    int32_t* table;
+    int max_pages, page, num_pages;
+    FastDiv by_page;
+    int32_t* ring;
+    uint32_t ring_size;
+    const int64_t* at;
+    int64_t* at_out;
+    int32_t *seq_lens, *held_out, *offsets, *positions, *slots;
+    int max_rows;
+    int32_t* counts;
+};
+
+// Last index in [0, n) whose entry is at most x (s[0] = 0 <= x, s ascending).
+__device__ __forceinline__ int pp_find(const int* s, int n, int x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s[mid] <= x) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+__global__ void __launch_bounds__(PP_THREADS) paged_plan_kernel(PlanArgs a) {
+    namespace cg = cooperative_groups;
+    __shared__ int s_row[PP_BATCH + 1], s_take[PP_BATCH + 1], s_back[PP_BATCH], s_ctx[PP_BATCH], s_held[PP_BATCH];
+    __shared__ long long s_part[PP_THREADS / 32][3];
+    __shared__ int s_most[2], s_refused;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const long long head = a.at[0], tail = a.at[1];
+    const bool sound = head >= 0 && tail >= head && tail - head <= (long long)a.ring_size;
+    const long long avail = sound ? tail - head : 0;
+    if (tid < 2) s_most[tid] = 0;
+    if (tid == 2) s_refused = 0;
+    int ctx[PP_EACH], fresh[PP_EACH], held[PP_EACH];
+    long long rows[PP_EACH], take[PP_EACH], back[PP_EACH], sum[3] = {0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < PP_EACH; ++i) {
+        const int b = tid * PP_EACH + i;
+        const bool there = b < a.batch;
+        ctx[i] = there ? a.ctx[b] : 0;
+        fresh[i] = there ? a.fresh[b] : 0;
+        held[i] = there ? a.held[b] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < PP_EACH; ++i) {
+        const long long want = (long long)ctx[i] + fresh[i];
+        const bool fits = fresh[i] > 0 && ctx[i] >= 0 && held[i] >= 0 && held[i] <= a.max_pages && want <= (long long)a.max_pages * a.page;
+        rows[i] = fits ? fresh[i] : 0;
+        take[i] = fits ? max(0ll, (want + a.page - 1) / a.page - held[i]) : 0;
+        back[i] = fresh[i] < 0 ? min(max(held[i], 0), a.max_pages) : 0;
+        sum[0] += rows[i];
+        sum[1] += take[i];
+        sum[2] += back[i];
+    }
+    long long before[3];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        long long v = sum[k];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += u;
+        }
+        before[k] = v - sum[k];
+        if (lane == 31) s_part[warp][k] = v;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+        for (int w = 0; w < warp; ++w) before[k] += s_part[w][k];
+    long long all_back = 0;
+    for (int w = 0; w < PP_THREADS / 32; ++w) all_back += s_part[w][2];
+    // admission; the largest sums among the admitted are the step's totals
+    bool ok[PP_EACH];
+    int refused = 0, most_rows = 0, most_take = 0;
+    long long first_row[PP_EACH], first_take[PP_EACH], first_back[PP_EACH];
+#pragma unroll
+    for (int i = 0; i < PP_EACH; ++i) {
+        first_row[i] = before[0];
+        first_take[i] = before[1];
+        first_back[i] = before[2];
+        before[0] += rows[i];
+        before[1] += take[i];
+        before[2] += back[i];
+        ok[i] = rows[i] > 0 && before[0] <= a.max_rows && before[1] <= avail;
+        if (ok[i]) {
+            most_rows = (int)before[0];
+            most_take = (int)before[1];
+        }
+        refused += fresh[i] > 0 && !ok[i];
+    }
+    most_rows = __reduce_max_sync(0xffffffffu, most_rows);
+    most_take = __reduce_max_sync(0xffffffffu, most_take);
+    refused = __reduce_add_sync(0xffffffffu, refused);
+    if (lane == 0) {
+        atomicMax(&s_most[0], most_rows);
+        atomicMax(&s_most[1], most_take);
+        if (refused) atomicAdd(&s_refused, refused);
+    }
+    __syncthreads();
+    const int all_rows = s_most[0], all_take = s_most[1];
+    // more pages than the ring has room for: a page held twice; none is put in
+    const int given = sound && all_back <= (long long)a.ring_size - avail ? (int)all_back : 0;
+#pragma unroll
+    for (int i = 0; i < PP_EACH; ++i) {
+        const int b = tid * PP_EACH + i;
+        if (b < a.batch) {
+            s_row[b] = (int)min(first_row[i], (long long)all_rows);
+            s_take[b] = (int)min(first_take[i], (long long)all_take);
+            s_back[b] = (int)first_back[i];
+            s_ctx[b] = ctx[i];
+            s_held[b] = held[i];
+        }
+    }
+    if (tid == 0) {
+        s_row[a.batch] = all_rows;
+        s_take[a.batch] = all_take;
+    }
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();                              // every block has read what the outputs may overwrite
+    const int rank = (int)cluster.block_rank(), nthreads = (int)cluster.num_blocks() * PP_THREADS, id = rank * PP_THREADS + tid;
+    if (rank == 0) {
+#pragma unroll
+        for (int i = 0; i < PP_EACH; ++i) {
+            const int b = tid * PP_EACH + i;
+            if (b >= a.batch) continue;
+            a.seq_lens[b] = fresh[i] < 0 ? 0 : ok[i] ? ctx[i] + fresh[i] : ctx[i];
+            a.held_out[b] = fresh[i] < 0 ? 0 : ok[i] ? held[i] + (int)take[i] : held[i];
+            a.offsets[b] = s_row[b];
+        }
+        if (tid == 0) {
+            a.offsets[a.batch] = all_rows;
+            a.at_out[0] = head + all_take;
+            a.at_out[1] = tail + given;
+            a.counts[0] = all_rows;
+            a.counts[1] = all_take;
+            a.counts[2] = given;
+            a.counts[3] = s_refused;
+        }
+    }
+    const uint32_t ring_head = sound ? (uint32_t)(head % a.ring_size) : 0, ring_tail = sound ? (uint32_t)(tail % a.ring_size) : 0;
+    auto ring_index = [&](uint32_t from, uint32_t j) {      // both below the ring's size
+        const uint32_t i = from + j;
+        return i >= a.ring_size ? i - a.ring_size : i;
+    };
+    for (int j = id; j < all_take; j += nthreads) {
+        const int b = pp_find(s_take, a.batch, j);
+        a.table[(int64_t)b * a.max_pages + s_held[b] + (j - s_take[b])] = a.ring[ring_index(ring_head, j)];
+    }
+    // the pages of the finished: behind the ring's end, never over entries that are being taken
+    for (int j = id; j < given; j += nthreads) {
+        const int b = pp_find(s_back, a.batch, j);
+        a.ring[ring_index(ring_tail, j)] = a.table[(int64_t)b * a.max_pages + (j - s_back[b])];
+    }
+    for (int r = id; r < a.max_rows; r += nthreads) {
+        int pos = -1, slot = -1;
+        if (r < all_rows) {
+            const int b = pp_find(s_row, a.batch, r);
+            pos = s_ctx[b] + (r - s_row[b]);
+            const int p = (int)a.by_page.div(pos), more = p - s_held[b];
+            const int id_of = more < 0 ? a.table[(int64_t)b * a.max_pages + p] : a.ring[ring_index(ring_head, s_take[b] + more)];
+            if ((uint32_t)id_of < (uint32_t)a.num_pages) slot = id_of * a.page + (pos - p * a.page);
+        }
+        a.positions[r] = pos;
+        a.slots[r] = slot;
+    }
+}
+
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" int b200_paged_plan(const int32_t* ctx_lens, const int32_t* new_lens, const int32_t* held, int batch, int32_t* page_table,
+                               int max_pages, int page, int num_pages, int32_t* free_ring, int ring_size, const int64_t* ring_at,
+                               int64_t* ring_at_out, int32_t* seq_lens, int32_t* held_out, int32_t* row_offsets,
+                               int32_t* positions, int32_t* slots, int max_rows, int32_t* counts) {
+    B200_REQUIRE(batch >= 0 && batch <= PP_BATCH, "paged_plan: batch must be in [0, %d]", PP_BATCH);
+    B200_REQUIRE(page >= 1 && max_pages >= 1 && num_pages >= 1, "paged_plan: bad page geometry");
+    B200_REQUIRE((int64_t)num_pages * page <= 0x7fffffff && (int64_t)max_pages * page <= 0x7fffffff,
+                 "paged_plan: num_pages * page and max_pages * page must fit in 31 bits");
+    B200_REQUIRE(ring_size >= num_pages, "paged_plan: the ring must have room for every page");
+    B200_REQUIRE(max_rows >= 0, "paged_plan: negative max_rows");
+    B200_REQUIRE(ring_at && ring_at_out && free_ring && row_offsets && counts, "paged_plan: null pointer");
+    B200_REQUIRE(batch == 0 || (ctx_lens && new_lens && held && page_table && seq_lens && held_out), "paged_plan: null pointer");
+    B200_REQUIRE(max_rows == 0 || (positions && slots), "paged_plan: null pointer");
+    PlanArgs a{ctx_lens, new_lens, held, batch, page_table, max_pages, page, num_pages, FastDiv(page), free_ring, (uint32_t)ring_size,
+               ring_at, ring_at_out, seq_lens, held_out, row_offsets, positions, slots, max_rows, counts};
+    const int blocks = max_rows > 2 * PP_THREADS || batch > 64 ? 8 : 1;
+    return launch_serve("paged_plan_kernel", paged_plan_kernel, dim3(blocks), dim3(PP_THREADS), 0, blocks, false, a);
+}
