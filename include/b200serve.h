@@ -21,8 +21,9 @@
  * 128 bytes from the page's start.  A token's row of hd elements (64 or 128) is cut in blocks of 32; element
  * 32 b + 4 g + i (b < hd/32, g < 8, i < 4) is nibble i, lowest first, of the row's 16-bit word g * (hd/32) + b.
  * kind 0 (Q4_0): a scale is one fp16 d, the value d * (code - 8); kind 1 (Q4_1): an fp16 pair d, m, the value
- * d * code + m.  Codes and scales are those of b200_quantize of the same kind, bit for bit, but for d and m beyond the
- * range of fp16, which are kept as +-65504 (every stored value is finite).  Slot s is token s % page of page s / page;
+ * d * code + m.  kind 0 holds the codes and scales of b200_quantize, bit for bit; kind 1 as well, but that its step is
+ * (max - min) * fp32(1/15), not a division: its last bit may differ and with it the code of a value on the border of two.  d and m beyond
+ * the range of fp16 are kept as +-65504 (every stored value is finite).  Slot s is token s % page of page s / page;
  * num_pages * page must fit in 31 bits. */
 #ifndef B200SERVE_H
 #define B200SERVE_H
@@ -91,8 +92,9 @@ int b200_kv4_fetch(const void* pages, int num_pages, int page, const int32_t* sl
  * tokens up to its own, with window > 0 the last `window` of them.  H a multiple of KV, hd 64 or 128.  max_rows: the most
  * rows of one sequence (it sizes the tiles; a sequence with more is still right).  page_table [batch, max_pages]; a length
  * beyond max_pages * page is cut to it; a page id outside [0, num_pages) reads as zeros.  A row before the sequence's first
- * token (more rows than tokens) is all zeros; rows of no sequence are left as they were.  fp32 accuracy: the queries and
- * probabilities travel as two fp16 parts (23 bits), codes are exact, sums are fp32.  hd and strides multiples of 4, q, out and pages
+ * token (more rows than tokens) is all zeros; rows of no sequence are left as they were.  fp32 accuracy: queries and
+ * probabilities travel as two fp16 parts that hold 2^-24 of the largest among them (of a query's elements; of 32 tokens' weights), codes are
+ * exact, sums are fp32.  hd and strides multiples of 4, q, out and pages
  * 16-byte aligned.  workspace: b200_attention_paged_kv4_workspace() bytes for the same H, KV, hd, max_rows (the batch
  * and the lengths do not matter). */
 int b200_attention_paged_kv4_workspace(int H, int KV, int hd, int max_rows, size_t* bytes);

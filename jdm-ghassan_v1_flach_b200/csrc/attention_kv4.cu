@@ -1,4 +1,29 @@
-// Attention of ragged rows over the 4-bit pages: the plain kernel, one block per row and head.
+// Attention of ragged rows over the 4-bit pages (b200serve.h), on mma.sync with the codes themselves as operands.
+//
+// The mathematics.  A key's element is d code + m (kind 1; kind 0 has m = -8 d) with d, m of its block of 32, so
+//   q . K = sum over blocks  d (sum of q code) + m (sum of q)         the last factor is a constant of the query
+//   o     = sum over keys    (p d) (code - 8) + p (m + 8 d)           p d goes to the tensor cores, the rest is one number per block
+// and the codes need no arithmetic at all: the bits of a code in the low end of an fp16 word are the subnormal code * 2^-24 (or, one nibble
+// up, code * 2^-20), exactly, and a product with them is exact too.  One AND makes a pair of operands.
+// Queries and p d travel as two fp16 parts in neighbouring columns.  The tensor cores cut what does not fit where they add, sixteen
+// times for one product; so the first part is a whole number of at most 2^11 (the power of two comes from the largest element of the
+// query, or the largest p d of the tile), whose sums of 32 with codes are whole numbers below 2^20 and never cut, and the second
+// the rest, at most 1/2, whose cuts are 2^-12 of those.  (With parts cut by significance instead, scores of +-10 were off by
+// 1e-5.)  Together they hold 2^-24 of the largest.  The values' sums start at -8 times the weights, a product with a constant: sums over thousands
+// of positive codes would have to lose most of their size again to p m (2e-6 of the output, where it is now below 5e-7).  An accumulator pair added up is one head's sum; what is beyond 32 dims or keys is
+// added in fp32 registers, the softmax statistics too.
+//   S^T [16 keys, 4 pairs x 2 parts] = K [16 keys, 16 dims] . q^T      keys as rows: a lane has a key's scores and scales together
+//   O^T [16 dims, 4 pairs x 2 parts] = V^T [16 dims, 16 keys] . (p d)^T, the weights' fragments turned by movmatrix
+// (pair: a query row and one of the heads that share the KV head).
+//
+// What bounds it: for single tokens the cache, 2 KV (hd/2 + 4 hd/32) bytes a token once (kind 1), with about 600 instructions of a
+// warp per 32 keys behind it - two thirds of what an SM can issue in the time the bytes take; for many rows the instructions.
+//
+// The split.  The lengths are on the device, so the grid is fixed (three blocks on every SM) and every block takes an equal share of all
+// (sequence, tile of pairs, KV head, 128 keys) units laid end to end, found from a prefix sum over the batch that
+// every block makes by itself.  What a share cuts off an item's ends goes to the workspace and is joined by a second, small kernel.
+// A warp takes 32 keys at a time for 4 or 8 pairs, from a ring of its own in shared memory that cp.async fills two tiles ahead;
+// where a sequence has more pairs the block's warps take different pairs instead of different keys.
 #include <algorithm>
 
 #include "serve.cuh"
@@ -6,6 +31,11 @@
 namespace b200 {
 
 constexpr int A4_WARPS = 4;
+constexpr int A4_THREADS = A4_WARPS * 32;
+constexpr int A4_KEYS = 32;                      // keys of a warp's step
+constexpr int A4_UNIT = 128;                     // keys of a unit
+constexpr int A4_STAGES = 3;
+constexpr int A4_BLOCKS = 3;                     // on an SM
 
 struct Kv4AttnArgs {
     const float* q;
@@ -18,65 +48,568 @@ struct Kv4AttnArgs {
     float* out;
     int64_t os;
     int batch, max_pages, page, H, KV, group;
-    FastDiv by_page;
+    FastDiv by_page, by_group, by_pairs;
     Kv4Page part;
     float scale;
     int window;
+    int across;                                  // warps that take different pairs; A4_WARPS / across take different keys
+    int pairs;                                   // of a block
+    float* piece;                                // [2 * blocks][pairs][hd + 2]: o, m, l of cut items
+    int4* item;                                  // [blocks]: pieces that follow the block's last one, sequence, tile, KV head
 };
 
+__device__ __forceinline__ void a4_mma0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ void a4_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t a4_turn(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t a4_pack(float low, float high) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(high), "f"(low));
+    return r;
+}
+__device__ __forceinline__ float a4_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t a4_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+template <int BYTES>
+__device__ __forceinline__ void a4_copy(uint32_t dst, const uint8_t* src, bool there) {   // zeros where there is nothing
+    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(there ? BYTES : 0) : "memory");
+}
+
+// A warp's stage: K codes, V codes, K scales, V scales of 32 keys.
 template <int HD, int KIND>
-__global__ void __launch_bounds__(A4_WARPS * 32) attn_kv4_plain_kernel(Kv4AttnArgs a) {
-    constexpr int NB = HD / 32, E = HD / 32;                 // elements per lane: element 32 e + lane
-    __shared__ float s_ml[A4_WARPS][2], s_o[A4_WARPS][HD];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int b = blockIdx.y; b < a.batch; b += gridDim.y) {
-        const int first = a.offsets ? a.offsets[b] : b, rows = a.offsets ? a.offsets[b + 1] - first : 1;
-        const int len = min(a.lens[b], a.max_pages * a.page);
-        for (int i = blockIdx.z; i < rows; i += gridDim.z) {
-            const int h = blockIdx.x, kv = h / a.group, pos = len - rows + i;
-            const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-            float q[E], o[E], m = -INFINITY, l = 0.0f;
-#pragma unroll
-            for (int e = 0; e < E; ++e) { q[e] = a.q[(first + i) * a.qs + (int64_t)h * HD + 32 * e + lane] * a.scale; o[e] = 0.0f; }
-            for (int j = lo + warp; j <= pos; j += A4_WARPS) {
-                const int p = (int)a.by_page.div(j), off = j - p * a.page, id = a.table[(int64_t)b * a.max_pages + p];
-                const bool there = (uint32_t)id < (uint32_t)a.num_pages;
-                const uint8_t* base = a.pages + (int64_t)(there ? id : 0) * a.part.bytes;
-                const int64_t row = (int64_t)kv * a.page + off;
-                auto value = [&](int64_t codes, int64_t scales, int e) {
-                    if (!there) return 0.0f;
-                    const int g = lane >> 2;
-                    const int c = (reinterpret_cast<const uint16_t*>(base + codes + row * (HD / 2))[g * NB + e] >> (4 * (lane & 3))) & 15;
-                    const uint16_t* s = reinterpret_cast<const uint16_t*>(base + scales) + (row * NB + e) * (KIND == 1 ? 2 : 1);
-                    return KIND == 1 ? half_bits_to_float(s[0]) * (float)c + half_bits_to_float(s[KIND]) : half_bits_to_float(s[0]) * (float)(c - 8);
-                };
-                float x = 0.0f;
-#pragma unroll
-                for (int e = 0; e < E; ++e) x += q[e] * value(0, a.part.k_scale, e);
-                x = warp_sum(x);
-                const float mn = fmaxf(m, x), f = expf(m - mn), w = expf(x - mn);
-                l = l * f + w;
-                m = mn;
-#pragma unroll
-                for (int e = 0; e < E; ++e) o[e] = o[e] * f + w * value(a.part.v_code, a.part.v_scale, e);
-            }
-            if (lane == 0) { s_ml[warp][0] = m; s_ml[warp][1] = l; }
-#pragma unroll
-            for (int e = 0; e < E; ++e) s_o[warp][32 * e + lane] = o[e];
-            __syncthreads();
-            if (warp == 0) {
-                float mm = -INFINITY, ll = 0.0f;
-                for (int w = 0; w < A4_WARPS; ++w) mm = fmaxf(mm, s_ml[w][0]);
-                for (int w = 0; w < A4_WARPS; ++w) ll += s_ml[w][1] == 0.0f ? 0.0f : s_ml[w][1] * expf(s_ml[w][0] - mm);
-                for (int e = 0; e < E; ++e) {
-                    float v = 0.0f;
-                    for (int w = 0; w < A4_WARPS; ++w) v += s_ml[w][1] == 0.0f ? 0.0f : s_o[w][32 * e + lane] * expf(s_ml[w][0] - mm);
-                    a.out[(first + i) * a.os + (int64_t)h * HD + 32 * e + lane] = ll == 0.0f ? 0.0f : v / ll;
-                }
-            }
-            __syncthreads();
+struct A4Stage {
+    static constexpr int NB = HD / 32;
+    static constexpr int ROW = HD / 2;           // bytes of a row's codes
+    static constexpr int SROW = NB * (KIND == 1 ? 4 : 2);
+    static constexpr int V = A4_KEYS * ROW, KS = 2 * V, VS = KS + A4_KEYS * SROW, BYTES = VS + A4_KEYS * SROW;
+    static constexpr int RING = A4_STAGES * BYTES;
+};
+
+// d and m of block b among the NB scales of a key held in registers.
+template <int KIND, int NB>
+struct A4Scales {
+    static constexpr int WORDS = KIND == 1 ? NB : NB / 2;
+    uint32_t w[WORDS];
+    __device__ __forceinline__ void load(const uint8_t* p) {
+        if (WORDS == 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(p);
+            w[0] = v.x; w[WORDS > 1 ? 1 : 0] = v.y; w[WORDS > 2 ? 2 : 0] = v.z; w[WORDS > 3 ? 3 : 0] = v.w;
+        } else if (WORDS == 2) {
+            const uint2 v = *reinterpret_cast<const uint2*>(p);
+            w[0] = v.x; w[WORDS > 1 ? 1 : 0] = v.y;
+        } else {
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
         }
     }
+    __device__ __forceinline__ void get(int b, float& d, float& m) const {
+        if (KIND == 1) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[b]));
+            d = f.x;
+            m = f.y;
+        } else {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[b / 2]));
+            d = b & 1 ? f.y : f.x;
+            m = -8.0f * d;
+        }
+    }
+};
+
+// A sequence's share of the units: rows, length, tiles of pairs, units of an item.
+struct A4Seq {
+    int first, rows, len, tiles, units;
+};
+__device__ __forceinline__ A4Seq a4_seq(const Kv4AttnArgs& a, int b) {
+    A4Seq s;
+    s.first = a.offsets ? a.offsets[b] : b;
+    s.rows = a.offsets ? max(a.offsets[b + 1] - s.first, 0) : 1;      // rows * group: q would not fit the device from 2^31 on
+    s.len = max(0, min(a.lens[b], a.max_pages * a.page));
+    s.tiles = (int)a.by_pairs.div((uint32_t)(s.rows * a.group + a.pairs - 1));
+    s.units = max(1, (s.len + A4_UNIT - 1) / A4_UNIT);
+    if (a.window > 0) s.units = (int)min((int64_t)s.units, ((int64_t)a.window + a.pairs / a.group + A4_UNIT + 1) / A4_UNIT + 1);
+    return s;
+}
+__device__ __forceinline__ int64_t a4_units(const Kv4AttnArgs& a, const A4Seq& s) { return (int64_t)s.tiles * a.KV * s.units; }
+
+// The keys that the pairs of one tile see, in units: the item's units are first .. first + units - 1, of which those from `end` on
+// (keys from key_end on) hold nothing.
+struct A4Range {
+    int first, key_end;
+};
+__device__ __forceinline__ A4Range a4_range(const Kv4AttnArgs& a, const A4Seq& s, int tile) {
+    const int last = min(s.rows - 1, (int)a.by_group.div((uint32_t)((tile + 1) * a.pairs - 1)));
+    A4Range r;
+    r.key_end = max(0, s.len - s.rows + last + 1);
+    r.first = max(0, (r.key_end + A4_UNIT - 1) / A4_UNIT - s.units);
+    return r;
+}
+
+template <int HD, int KIND, int NT>
+__global__ void __launch_bounds__(A4_THREADS, A4_BLOCKS) attn_kv4_kernel(const __grid_constant__ Kv4AttnArgs a) {
+    using ST = A4Stage<HD, KIND>;
+    constexpr int NB = ST::NB;
+    constexpr uint32_t LOW = 0x000F000Fu, UP = 0x00F000F0u;      // code * 2^-24, code * 2^-20
+    constexpr uint32_t LESS_8 = 0x80088008u, LESS_8_UP = 0x80808080u;        // -8 of each
+    constexpr float ROUND = 12582912.0f;                         // 1.5 * 2^23
+    extern __shared__ __align__(128) uint8_t a4_ring[];
+    __shared__ int64_t s_sum[A4_WARPS], s_rest;
+    __shared__ int s_b;
+    __shared__ float s_ml[A4_WARPS][4 * NT][2];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    asm volatile("griddepcontrol.launch_dependents;");
+
+    // ---- this block's share of the units ----
+    const int each = (a.batch + A4_THREADS - 1) / A4_THREADS, b0 = threadIdx.x * each;
+    int64_t mine = 0;
+    for (int b = b0; b < min(a.batch, b0 + each); ++b) mine += a4_units(a, a4_seq(a, b));
+    int64_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+    }
+    if (lane == 31) s_sum[warp] = upto;
+    __syncthreads();
+    int64_t all = 0;
+#pragma unroll
+    for (int w = 0; w < A4_WARPS; ++w) {
+        if (w < warp) upto += s_sum[w];
+        all += s_sum[w];
+    }
+    const int64_t per = (all + gridDim.x - 1) / gridDim.x;
+    int64_t u = (int64_t)blockIdx.x * per;
+    const int64_t u_end = min(all, u + per);
+    if (threadIdx.x == 0) a.item[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (u >= u_end) return;
+    if (upto - mine <= u && u < upto) {
+        int64_t rest = u - (upto - mine);
+        int b = b0;
+        for (;; ++b) {
+            const int64_t n = a4_units(a, a4_seq(a, b));
+            if (rest < n) break;
+            rest -= n;
+        }
+        s_b = b;
+        s_rest = rest;
+    }
+    __syncthreads();
+    int b = s_b;
+    int64_t rest = s_rest;
+    A4Seq seq = a4_seq(a, b);
+
+    const bool wide = a.page % A4_KEYS == 0;                     // a warp's keys lie in one page
+    const int side = warp % a.across, step0 = warp / a.across, step = A4_WARPS / a.across * A4_KEYS;
+    uint8_t* ring = a4_ring + warp * ST::RING;
+    const uint32_t ring_at = a4_smem(ring);
+
+    while (true) {
+        const int64_t item = rest / seq.units;
+        const int i0 = (int)(rest - item * seq.units), i1 = (int)min((int64_t)seq.units, i0 + (u_end - u));
+        const int kv = (int)(item / seq.tiles), tile = (int)(item - (int64_t)kv * seq.tiles);
+        const A4Range range = a4_range(a, seq, tile);
+        const int kbeg = (range.first + i0) * A4_UNIT, kend = (int)min((int64_t)range.key_end, ((int64_t)range.first + i1) * A4_UNIT);
+        const int32_t* table = a.table + (int64_t)b * a.max_pages;
+        const int pair0 = tile * a.pairs + side * 4 * NT, npairs = seq.rows * a.group;
+
+        // ---- one tile of 32 keys into stage s ----
+        auto page_of = [&](int k) { return k < kend ? table[a.by_page.div(wide ? k : min(k + lane, kend - 1))] : -1; };
+        auto issue = [&](int s, int k, int id) {
+            constexpr int CH = ST::ROW / 16, PER = 32 / CH;      // 16-byte pieces of a row, keys per round
+            const uint32_t dst = ring_at + s * ST::BYTES;
+            const bool there = (uint32_t)id < (uint32_t)a.num_pages;
+            const int key = min(k + (wide ? 0 : lane), kend - 1);
+            const int off = key - (int)a.by_page.div(key) * a.page;
+            const int64_t at = (int64_t)(there ? id : 0) * a.part.bytes;           // of the page
+            const int64_t row = (int64_t)kv * a.page + off;                              // of the tile's first key, or the lane's
+#pragma unroll
+            for (int i = 0; i < A4_KEYS / PER; ++i) {
+                const int key_of = i * PER + lane / CH;
+                int64_t src;
+                bool ok = k + key_of < kend;
+                if (wide) {
+                    src = at + (row + key_of) * ST::ROW;
+                    ok = ok && there;
+                } else {
+                    src = __shfl_sync(0xffffffffu, at + row * ST::ROW, key_of);
+                    ok = __shfl_sync(0xffffffffu, there, key_of) && ok;
+                }
+                if (!ok) src = 0;
+                const uint8_t* p = a.pages + src + lane % CH * 16;
+                // K rows in the order in which the fragments take them, V rows as they come, their pieces swapped so that four rows
+                // apart by one miss each other's banks
+                const int kr = (key_of & 24) + 2 * (key_of & 3) + ((key_of >> 2) & 1);
+                const int vc = HD == 128 ? lane % CH ^ (key_of & 2) : lane % CH;
+                a4_copy<16>(dst + kr * ST::ROW + lane % CH * 16, p, ok);
+                a4_copy<16>(dst + ST::V + key_of * ST::ROW + vc * 16, p + a.part.v_code, ok);
+            }
+            const bool ok = k + lane < kend && there;
+            const uint8_t* p = a.pages + (ok ? at + (row + (wide ? lane : 0)) * ST::SROW : 0);
+            a4_copy<ST::SROW>(dst + ST::KS + lane * ST::SROW, p + a.part.k_scale, ok);
+            a4_copy<ST::SROW>(dst + ST::VS + lane * ST::SROW, p + a.part.v_scale, ok);
+        };
+        auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+
+        int k = kbeg + step0 * A4_KEYS;
+#pragma unroll
+        for (int s = 0; s < A4_STAGES - 1; ++s) {
+            if (k + s * step < kend) issue(s, k + s * step, page_of(k + s * step));
+            commit();
+        }
+        int next_id = page_of(k + (A4_STAGES - 1) * step);
+
+        // ---- queries: parts of q 2^e as B fragments, sums of each block ----
+        uint32_t qf[NT][NB][2][2];
+        float qsum[NT][NB], unit[NT];
+        int lim[NT], from[NT];
+        int all_see = 0x7fffffff, none_before = 0;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int p = pair0 + 4 * j + (g >> 1);
+            const bool live = p < npairs;
+            const int row = live ? (int)a.by_group.div(p) : 0;
+            const float* q = a.q + (int64_t)(seq.first + row) * a.qs + ((int64_t)kv * a.group + (live ? p - row * a.group : 0)) * HD + 8 * t;
+            float x[NB][8], top = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
+                if (live) {
+                    lo = __ldg(reinterpret_cast<const float4*>(q + 32 * n));
+                    hi = __ldg(reinterpret_cast<const float4*>(q + 32 * n + 4));
+                }
+                x[n][0] = lo.x; x[n][1] = lo.y; x[n][2] = lo.z; x[n][3] = lo.w;
+                x[n][4] = hi.x; x[n][5] = hi.y; x[n][6] = hi.z; x[n][7] = hi.w;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[n][i]));
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int e = max((int)(__float_as_uint(top) >> 23), 14);             // top < 2^(e - 126)
+            const float mul = __uint_as_float((uint32_t)(264 - e) << 23);         // 2^(137 - e): top * mul < 2^11
+            const float back = __uint_as_float((uint32_t)(e == 255 ? 254 : e) << 23) * 16384.0f;     // 2^24 / mul
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                float sum = ((x[n][0] + x[n][1]) + (x[n][2] + x[n][3])) + ((x[n][4] + x[n][5]) + (x[n][6] + x[n][7]));
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                qsum[j][n] = __shfl_sync(0xffffffffu, sum * mul * 0x1p-24f, 8 * t);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    // nibble i of two words, elements i and 4 + i; an odd nibble's codes come 16 times too large
+                    const float f = i & 1 ? 0.0625f : 1.0f, u0 = x[n][i] * mul, u1 = x[n][4 + i] * mul, h0 = rintf(u0), h1 = rintf(u1);
+                    qf[j][n][i >> 1][i & 1] = g & 1 ? a4_pack((u0 - h0) * f, (u1 - h1) * f) : a4_pack(h0 * f, h1 * f);
+                }
+            }
+            unit[j] = __shfl_sync(0xffffffffu, back, 8 * t) * (a.scale * 1.4426950408889634f);       // to powers of two
+            const int pt = pair0 + 4 * j + t;
+            const int pos = pt < npairs ? seq.len - seq.rows + (int)a.by_group.div(pt) : 0x7ffffffe;
+            lim[j] = pos + 1;
+            from[j] = a.window > 0 && pt < npairs ? max(0, pos - a.window + 1) : 0;
+            all_see = min(all_see, lim[j]);
+            none_before = max(none_before, from[j]);
+        }
+        all_see = __reduce_min_sync(0xffffffffu, all_see);
+        none_before = __reduce_max_sync(0xffffffffu, none_before);
+
+        float o[NT][2 * NB][2], bias[NT][NB], m[NT], l[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            m[j] = -INFINITY;
+            l[j] = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                bias[j][n] = 0.0f;
+                o[j][2 * n][0] = o[j][2 * n][1] = o[j][2 * n + 1][0] = o[j][2 * n + 1][1] = 0.0f;
+            }
+        }
+        const int kk = (g >> 1) + 4 * (g & 1);                    // key (of 8) that fragment row g is
+
+        for (int s = 0; k < kend; k += step, s = s + 1 == A4_STAGES ? 0 : s + 1) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(A4_STAGES - 2) : "memory");
+            __syncwarp();                                         // this tile is here, and the one before it is read
+            {
+                const int ahead = k + (A4_STAGES - 1) * step;
+                if (ahead < kend) issue(s == 0 ? A4_STAGES - 1 : s - 1, ahead, next_id);
+                commit();
+                next_id = page_of(ahead + step);
+            }
+            const uint8_t* st = ring + s * ST::BYTES;
+
+            // ---- scores ----
+            float x[NT][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t w[2][NB];                                // of key rows g and g + 8: nibble i of word t's two halves
+                A4Scales<KIND, NB> sc[2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const uint8_t* p = st + (16 * h + 8 * r + g) * ST::ROW;
+                    if (HD == 128) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(p + 16 * t);
+                        w[r][0] = __byte_perm(v.x, v.z, 0x5410);
+                        w[r][1] = __byte_perm(v.x, v.z, 0x7632);
+                        w[r][NB > 2 ? 2 : 0] = __byte_perm(v.y, v.w, 0x5410);
+                        w[r][NB > 2 ? 3 : 0] = __byte_perm(v.y, v.w, 0x7632);
+                    } else {
+                        const uint2 v = *reinterpret_cast<const uint2*>(p + 8 * t);
+                        w[r][0] = __byte_perm(v.x, v.y, 0x5410);
+                        w[r][1] = __byte_perm(v.x, v.y, 0x7632);
+                    }
+                    sc[r].load(st + ST::KS + (16 * h + 8 * r + kk) * ST::SROW);
+                }
+#pragma unroll
+                for (int j = 0; j < NT; ++j) x[j][2 * h] = x[j][2 * h + 1] = 0.0f;
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    const uint32_t s0 = w[0][n] >> 8, s1 = w[1][n] >> 8;
+                    float d0, m0, d1, m1;
+                    sc[0].get(n, d0, m0);
+                    sc[1].get(n, d1, m1);
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        float c[4];
+                        a4_mma0(c, w[0][n] & LOW, w[1][n] & LOW, w[0][n] & UP, w[1][n] & UP, qf[j][n][0][0], qf[j][n][0][1]);
+                        a4_mma(c, s0 & LOW, s1 & LOW, s0 & UP, s1 & UP, qf[j][n][1][0], qf[j][n][1][1]);
+                        x[j][2 * h] = fmaf(m0, qsum[j][n], fmaf(d0, c[0] + c[1], x[j][2 * h]));
+                        x[j][2 * h + 1] = fmaf(m1, qsum[j][n], fmaf(d1, c[2] + c[3], x[j][2 * h + 1]));
+                    }
+                }
+            }
+            // ---- softmax ----
+            const bool cut = k + A4_KEYS > all_see || k < none_before;
+            bool grown = false;
+            float top[NT], here[NT];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[j][i] *= unit[j];
+                    if (cut) {
+                        const int key = k + 8 * i + kk;
+                        if (key >= lim[j] || key < from[j]) x[j][i] = -INFINITY;
+                    }
+                }
+                float v = fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3]));
+                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+                here[j] = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+                top[j] = fmaxf(m[j], here[j]);
+                grown |= top[j] != m[j];
+            }
+            if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const float f = m[j] == top[j] ? 1.0f : a4_exp2(m[j] - top[j]);
+                    m[j] = top[j];
+                    l[j] *= f;
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) {
+                        bias[j][n] *= f;
+                        o[j][2 * n][0] *= f; o[j][2 * n][1] *= f;
+                        o[j][2 * n + 1][0] *= f; o[j][2 * n + 1][1] *= f;
+                    }
+                }
+            }
+            // ---- values ----
+            A4Scales<KIND, NB> sv[4];
+            uint32_t top_d = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                sv[i].load(st + ST::VS + (8 * i + kk) * ST::SROW);
+#pragma unroll
+                for (int n = 0; n < A4Scales<KIND, NB>::WORDS; ++n) {
+                    const uint32_t mag = sv[i].w[n] & 0x7FFF7FFFu;
+                    top_d = KIND == 1 ? max(top_d, mag & 0xFFFFu) : __vmaxu2(top_d, mag);
+                }
+            }
+            if (KIND == 0) top_d = max(top_d & 0xFFFFu, top_d >> 16);
+            const float largest = half_bits_to_float((uint16_t)__reduce_max_sync(0xffffffffu, top_d));
+            float pg[NT][4], shrink[NT];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const float base = m[j] == -INFINITY ? 0.0f : m[j];
+                // every p d of the tile < 2^(e - 126) (or a rounding above)
+                const uint32_t e = max(__float_as_uint(a4_exp2(here[j] - base) * largest) >> 23, 11u);
+                const float grow = __uint_as_float((264u - e) << 23);             // 2^(137 - e): p d grow < 2^11
+                shrink[j] = __uint_as_float((14u + e) << 23);                     // 2^24 / grow
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[j][i] = a4_exp2(x[j][i] - base);
+                l[j] += (x[j][0] + x[j][1]) + (x[j][2] + x[j][3]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) pg[j][i] = x[j][i] * grow;
+            }
+            uint32_t vx[8], vy[8];                                // of keys t, t + 4, .. t + 28: the words of dims 4 g .. 4 g + 3
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint8_t* p = st + ST::V + (4 * i + t) * ST::ROW;
+                if (HD == 128) {
+                    const uint2 v = *reinterpret_cast<const uint2*>(p + (((g >> 1) ^ (t & 2)) * 16 + (g & 1) * 8));
+                    vx[i] = v.x;
+                    vy[i] = v.y;
+                } else {
+                    vx[i] = *reinterpret_cast<const uint32_t*>(p + 4 * g);
+                    vy[i] = 0;
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                uint32_t pb[NT][4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float d, mn;
+                    sv[i].get(n, d, mn);
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        const float whole = fmaf(pg[j][i], d, ROUND) - ROUND;     // to the nearest whole number
+                        pb[j][i] = a4_turn(a4_pack(whole, fmaf(pg[j][i], d, -whole)));
+                        if (KIND == 1) bias[j][n] = fmaf(x[j][i], fmaf(8.0f, d, mn), bias[j][n]);
+                    }
+                }
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    w[i] = n < 2 ? __byte_perm(vx[2 * i], vx[2 * i + 1], n & 1 ? 0x7632 : 0x5410) : __byte_perm(vy[2 * i], vy[2 * i + 1], n & 1 ? 0x7632 : 0x5410);
+                float eights[NT][4];
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    a4_mma0(eights[j], LESS_8, LESS_8_UP, LESS_8, LESS_8_UP, pb[j][0], pb[j][1]);
+                    a4_mma(eights[j], LESS_8, LESS_8_UP, LESS_8, LESS_8_UP, pb[j][2], pb[j][3]);
+                }
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        float c[4] = {eights[j][0], eights[j][1], eights[j][2], eights[j][3]};
+                        a4_mma(c, w[0] & LOW, w[0] & UP, w[1] & LOW, w[1] & UP, pb[j][0], pb[j][1]);
+                        a4_mma(c, w[2] & LOW, w[2] & UP, w[3] & LOW, w[3] & UP, pb[j][2], pb[j][3]);
+                        o[j][2 * n + v][0] = fmaf(c[0] + c[1], shrink[j], o[j][2 * n + v][0]);
+                        o[j][2 * n + v][1] = fmaf(c[2] + c[3], shrink[j], o[j][2 * n + v][1]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] >>= 8;
+                }
+            }
+        }
+        // ---- the lanes' sums, then the warps' ----
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();                                          // the rings become the warps' results
+        float* res = reinterpret_cast<float*>(a4_ring);           // [warp][pair][HD]
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+#pragma unroll
+            for (int sh = 4; sh < 32; sh <<= 1) {
+                l[j] += __shfl_xor_sync(0xffffffffu, l[j], sh);
+#pragma unroll
+                for (int n = 0; n < NB; ++n) bias[j][n] += __shfl_xor_sync(0xffffffffu, bias[j][n], sh);
+            }
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+                *reinterpret_cast<float4*>(res + (warp * 4 * NT + 4 * j + t) * HD + 32 * n + 4 * g) =
+                    make_float4(o[j][2 * n][0] + bias[j][n], fmaf(o[j][2 * n][1], 0.0625f, bias[j][n]), o[j][2 * n + 1][0] + bias[j][n],
+                                fmaf(o[j][2 * n + 1][1], 0.0625f, bias[j][n]));
+            if (g == 0) {
+                s_ml[warp][4 * j + t][0] = m[j];
+                s_ml[warp][4 * j + t][1] = l[j];
+            }
+        }
+        __syncthreads();
+        const bool whole = i0 == 0 && i1 == seq.units;
+        const int slot = 2 * blockIdx.x + (i0 == 0);
+        const int npr = min(a.pairs, npairs - tile * a.pairs);
+        for (int i = threadIdx.x; i < npr * (HD / 4); i += A4_THREADS) {
+            const int p = i / (HD / 4), c = i % (HD / 4) * 4, sd = p / (4 * NT), pp = p % (4 * NT);
+            float mm = -INFINITY, ll = 0.0f;
+            for (int w = sd; w < A4_WARPS; w += a.across) mm = fmaxf(mm, s_ml[w][pp][0]);
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int w = sd; w < A4_WARPS; w += a.across) {
+                const float lw = s_ml[w][pp][1];
+                const float f = s_ml[w][pp][0] == -INFINITY && lw == 0.0f ? 0.0f : a4_exp2(s_ml[w][pp][0] - mm);
+                const float4 v = *reinterpret_cast<const float4*>(res + (w * 4 * NT + pp) * HD + c);
+                ll += lw * f;
+                acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+            }
+            if (whole) {
+                const int of = tile * a.pairs + p, row = (int)a.by_group.div(of);
+                const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+                float* dst = a.out + (int64_t)(seq.first + row) * a.os + ((int64_t)kv * a.group + (of - row * a.group)) * HD + c;
+                *reinterpret_cast<float4*>(dst) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+            } else {
+                float* dst = a.piece + ((int64_t)slot * a.pairs + p) * (HD + 4);
+                *reinterpret_cast<float4*>(dst + c) = acc;
+                if (c == 0) { dst[HD] = mm; dst[HD + 1] = ll; }
+            }
+        }
+        if (i0 == 0 && !whole && threadIdx.x == 0) {
+            const int64_t more = seq.units - i1;                  // units of this item in the blocks that follow
+            a.item[blockIdx.x] = make_int4((int)((more + per - 1) / per), b, tile, kv);
+        }
+        u += i1 - i0;
+        if (u >= u_end) return;
+        rest += i1 - i0;
+        if (rest >= a4_units(a, seq)) {
+            rest = 0;
+            do seq = a4_seq(a, ++b); while (seq.rows == 0);       // there is one: units are left
+        }
+        __syncthreads();                                          // the results are read, the rings may fill again
+    }
+}
+
+// Items that a block began and others went on with: one block each.
+template <int HD>
+__global__ void __launch_bounds__(A4_THREADS) attn_kv4_join_kernel(const __grid_constant__ Kv4AttnArgs a) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int4 it = __ldcg(a.item + blockIdx.x);
+    if (it.x == 0) return;
+    const A4Seq seq = a4_seq(a, it.y);
+    const int first = it.z * a.pairs, npr = min(a.pairs, seq.rows * a.group - first);
+    // piece i: the block's own second slot, then the first slots of those behind it
+    auto piece = [&](int i, int p) { return a.piece + ((int64_t)(2 * (blockIdx.x + i) + (i == 0)) * a.pairs + p) * (HD + 4); };
+    for (int i = blockIdx.y * A4_THREADS + threadIdx.x; i < npr * (HD / 4); i += gridDim.y * A4_THREADS) {
+        const int p = i / (HD / 4), c = i % (HD / 4) * 4;
+        float mm = -INFINITY, ll = 0.0f;
+        for (int n = 0; n <= it.x; ++n) mm = fmaxf(mm, __ldcg(piece(n, p) + HD));
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int n = 0; n <= it.x; ++n) {
+            const float* s = piece(n, p);
+            const float ln = __ldcg(s + HD + 1), mn = __ldcg(s + HD);
+            const float f = mn == -INFINITY && ln == 0.0f ? 0.0f : a4_exp2(mn - mm);
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(s + c));
+            ll += ln * f;
+            acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+        }
+        const int row = (int)a.by_group.div(first + p);
+        const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+        float* dst = a.out + (int64_t)(seq.first + row) * a.os + ((int64_t)it.w * a.group + (first + p - row * a.group)) * HD + c;
+        *reinterpret_cast<float4*>(dst) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    }
+}
+
+// Pairs of a warp (4 or 8) and warps that take different pairs, from the most pairs that a sequence has for a KV head.
+static void a4_shape(int64_t most, int& nt, int& across) {
+    nt = most <= 4 ? 1 : 2;
+    across = most <= 8 ? 1 : most <= 16 ? 2 : 4;
+}
+static int a4_blocks() { return A4_BLOCKS * num_sms(); }
+
+template <int HD, int KIND, int NT>
+static int launch_a4(const Kv4AttnArgs& a, int blocks) {
+    auto kern = attn_kv4_kernel<HD, KIND, NT>;
+    constexpr int smem = A4_WARPS * A4Stage<HD, KIND>::RING;
+    if (smem > 48 * 1024) B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    return launch_serve("attn_kv4_kernel", kern, dim3(blocks), dim3(A4_THREADS), smem, 1, false, a);
 }
 
 }  // namespace b200
@@ -90,7 +623,9 @@ int b200_attention_paged_kv4_workspace(int H, int KV, int hd, int max_rows, size
     if (rc) return rc;
     B200_REQUIRE(bytes, "attention_paged_kv4_workspace: null pointer");
     B200_REQUIRE(H >= 1 && H % KV == 0 && max_rows >= 1, "attention_paged_kv4_workspace: H must be a positive multiple of KV, max_rows positive");
-    *bytes = 16;
+    int nt, across;
+    a4_shape((int64_t)max_rows * (H / KV), nt, across);
+    *bytes = (size_t)a4_blocks() * (sizeof(int4) + (size_t)2 * 4 * nt * across * (hd + 4) * sizeof(float));
     return B200_OK;
 }
 
@@ -103,7 +638,7 @@ int b200_attention_paged_kv4(const float* q, int64_t q_stride, const int32_t* ro
     int rc = kv4_check(who, num_pages, page, KV, hd, kind);
     if (rc) return rc;
     B200_REQUIRE(H >= 1 && H % KV == 0, "%s: H must be a positive multiple of KV", who);
-    B200_REQUIRE(max_rows >= 1 && max_pages >= 1 && (int64_t)max_pages * page <= 0x7fffffff, "%s: bad max_rows or max_pages", who);
+    B200_REQUIRE(max_rows >= 1 && max_pages >= 1 && (int64_t)max_pages * page <= 0x7fffff00, "%s: bad max_rows or max_pages", who);
     B200_REQUIRE(q && pages && page_table && seq_lens && out && workspace, "%s: null pointer", who);
     B200_REQUIRE(aligned16(q) && aligned16(out) && aligned16(pages) && aligned16(workspace) && q_stride % 4 == 0 && out_stride % 4 == 0,
                  "%s: q, out, pages and workspace must be 16-byte aligned, strides multiples of 4", who);
@@ -112,12 +647,22 @@ int b200_attention_paged_kv4(const float* q, int64_t q_stride, const int32_t* ro
     rc = b200_attention_paged_kv4_workspace(H, KV, hd, max_rows, &need);
     if (rc) return rc;
     B200_REQUIRE(workspace_bytes >= need, "%s: the workspace has %zu bytes of %zu", who, workspace_bytes, need);
+    int nt, across;
+    a4_shape((int64_t)max_rows * (H / KV), nt, across);
+    const int blocks = a4_blocks();
     Kv4AttnArgs a{q, q_stride, row_offsets, static_cast<const uint8_t*>(pages), num_pages, page_table, seq_lens, out, out_stride, batch,
-                  max_pages, page, H, KV, H / KV, FastDiv(page), Kv4Page(page, KV, hd, kind), scale, window};
-    const dim3 grid(H, std::min(batch, 65535), std::min(max_rows, 65535)), block(A4_WARPS * 32);
-    auto kern = hd == 64 ? (kind == 1 ? attn_kv4_plain_kernel<64, 1> : attn_kv4_plain_kernel<64, 0>)
-                         : (kind == 1 ? attn_kv4_plain_kernel<128, 1> : attn_kv4_plain_kernel<128, 0>);
-    return launch_serve("attn_kv4_plain_kernel", kern, grid, block, 0, 1, false, a);
+                  max_pages, page, H, KV, H / KV, FastDiv(page), FastDiv(H / KV), FastDiv(4 * nt * across), Kv4Page(page, KV, hd, kind), scale, window, across, 4 * nt * across,
+                  reinterpret_cast<float*>(static_cast<int4*>(workspace) + blocks), static_cast<int4*>(workspace)};
+    if (hd == 64)
+        rc = kind == 1 ? (nt == 1 ? launch_a4<64, 1, 1>(a, blocks) : launch_a4<64, 1, 2>(a, blocks))
+                       : (nt == 1 ? launch_a4<64, 0, 1>(a, blocks) : launch_a4<64, 0, 2>(a, blocks));
+    else
+        rc = kind == 1 ? (nt == 1 ? launch_a4<128, 1, 1>(a, blocks) : launch_a4<128, 1, 2>(a, blocks))
+                       : (nt == 1 ? launch_a4<128, 0, 1>(a, blocks) : launch_a4<128, 0, 2>(a, blocks));
+    if (rc) return rc;
+    const dim3 grid(blocks, std::max(1, a.pairs * (hd / 4) / A4_THREADS));
+    return hd == 64 ? launch_serve("attn_kv4_join_kernel", attn_kv4_join_kernel<64>, grid, dim3(A4_THREADS), 0, 1, true, a)
+                    : launch_serve("attn_kv4_join_kernel", attn_kv4_join_kernel<128>, grid, dim3(A4_THREADS), 0, 1, true, a);
 }
 
 }  // extern "C"

@@ -1,8 +1,10 @@
 // Rows of keys and values into the 4-bit pages and back (layout: b200serve.h).
 //
-// The rule is b200_quantize's for kinds 0 and 1, one correctly rounded fp32 operation at a time, so that codes and
-// scales are the same bits; a scale or minimum beyond the range of fp16 is kept at its largest value, because an infinite one
-// would make a NaN of every code 0, and of every masked probability in the attention over these pages.
+// The rule is b200_quantize's for kinds 0 and 1, one correctly rounded fp32 operation at a time, but for two things.  The step of
+// kind 1 is (max - min) times fp32(1/15) where that divides by 15: every new token pays for it, and the quotient's last bit
+// decides only for a value on the border of two codes.  And a scale or minimum beyond the range of fp16 is kept at its largest
+// value, because an infinite one would make a NaN of every code 0, and of every masked probability in the attention over these
+// pages.
 //
 // What bounds both: the fp32 rows (8 KV hd bytes a token), a quarter of that again for the pages' lines.  Eight lanes share a block of 32, each
 // with the four elements of one 16-bit word, so a warp reads 512 consecutive bytes and the block's statistics take three
@@ -97,7 +99,7 @@ __global__ void __launch_bounds__(KC_THREADS) kv4_store_kernel(Kv4Rows a) {
                     lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, s));
                     hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, s));
                 }
-                const float d = __fdiv_rn(__fsub_rn(hi, lo), 15.0f), inv = d > 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
+                const float d = __fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f), inv = d > 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) code |= (uint32_t)min(max((int)roundf(__fmul_rn(__fsub_rn(x[i], lo), inv)), 0), 15) << (4 * i);
                 scale = kc_half(d) | (kc_half(lo) << 16);

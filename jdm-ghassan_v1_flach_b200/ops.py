@@ -13,4 +13,5 @@ def __getattr__(name):
     L = lib()
     if sym not in L.protos:
         raise AttributeError(f"no such op: {name}")
-    return lambda *args: L.call(sym, *args)
+    fn = globals()[name] = getattr(L, sym)
+    return fn

@@ -22,7 +22,7 @@ def quantize(x, kind):
     b = np.where(bad, f(0), b)
     with np.errstate(over="ignore", divide="ignore", invalid="ignore"):
         low = b.min(-1, keepdims=True) if kind == 1 else f(0)
-        d = (b.max(-1, keepdims=True) - low) / f(15) if kind == 1 else np.abs(b).max(-1, keepdims=True) / f(8)
+        d = (b.max(-1, keepdims=True) - low) * (f(1) / f(15)) if kind == 1 else np.abs(b).max(-1, keepdims=True) / f(8)
         inv = np.where(d > 0, f(1) / d, f(0))
         t = ((b - low) * inv).astype(np.float64)
         r = np.copysign(np.floor(np.abs(t) + 0.5), t)
