@@ -33,9 +33,19 @@ namespace b200 {
 constexpr int A4_WARPS = 4;
 constexpr int A4_THREADS = A4_WARPS * 32;
 constexpr int A4_KEYS = 32;                      // keys of a warp's step
-constexpr int A4_UNIT = 128;                     // keys of a unit
-constexpr int A4_STAGES = 3;
-constexpr int A4_BLOCKS = 3;                     // on an SM
+#ifndef A4_ITEM
+#define A4_ITEM 2
+#define A4_LEAST 2
+#endif
+#ifndef A4_S1
+#define A4_S1 2
+#define A4_B1 4
+#define A4_S2 3
+#define A4_B2 3
+#endif
+// Stages of a warp's ring and blocks of an SM, by the warp's tiles of four pairs.
+__host__ __device__ constexpr int a4_stages(int nt) { return nt == 1 ? A4_S1 : A4_S2; }
+__host__ __device__ constexpr int a4_resident(int nt) { return nt == 1 ? A4_B1 : A4_B2; }
 
 struct Kv4AttnArgs {
     const float* q;
@@ -52,25 +62,36 @@ struct Kv4AttnArgs {
     Kv4Page part;
     float scale;
     int window;
-    int across;                                  // warps that take different pairs; A4_WARPS / across take different keys
-    int pairs;                                   // of a block
-    float* piece;                                // [2 * blocks][pairs][hd + 2]: o, m, l of cut items
-    int4* item;                                  // [blocks]: pieces that follow the block's last one, sequence, tile, KV head
+    int across;                                  // warps of a worker: they take different pairs
+    int pairs;                                   // of a worker
+    float* piece;                                // [2 * workers][pairs][hd + 4]: o, m, l of cut items
+    struct A4Item* item;                         // [workers]
+};
+// What a worker began and left to those behind it: how many of them (0: nothing), the sequence's first row, the tile's first pair
+// and its number of pairs, the KV head.
+struct __align__(16) A4Item {
+    int more, first, pair, live, kv, pad[3];
 };
 
 __device__ __forceinline__ void a4_mma0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ void a4_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// from (c0, c1) in both row halves
+__device__ __forceinline__ void a4_mma_from(float (&d)[4], float c0, float c1, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+}
 __device__ __forceinline__ uint32_t a4_turn(uint32_t x) {
     uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
 __device__ __forceinline__ uint32_t a4_pack(float low, float high) {
@@ -85,6 +106,11 @@ __device__ __forceinline__ float a4_exp2(float x) {
 }
 __device__ __forceinline__ uint32_t a4_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 template <int BYTES>
+__device__ __forceinline__ void a4_copy(uint32_t dst, const uint8_t* src) {
+    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+template <int BYTES>
 __device__ __forceinline__ void a4_copy(uint32_t dst, const uint8_t* src, bool there) {   // zeros where there is nothing
     if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
     else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(there ? BYTES : 0) : "memory");
@@ -97,7 +123,6 @@ struct A4Stage {
     static constexpr int ROW = HD / 2;           // bytes of a row's codes
     static constexpr int SROW = NB * (KIND == 1 ? 4 : 2);
     static constexpr int V = A4_KEYS * ROW, KS = 2 * V, VS = KS + A4_KEYS * SROW, BYTES = VS + A4_KEYS * SROW;
-    static constexpr int RING = A4_STAGES * BYTES;
 };
 
 // d and m of block b among the NB scales of a key held in registers.
@@ -124,7 +149,7 @@ struct A4Scales {
         } else {
             const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[b / 2]));
             d = b & 1 ? f.y : f.x;
-            m = -8.0f * d;
+            m = 0.0f;
         }
     }
 };
@@ -139,11 +164,11 @@ __device__ __forceinline__ A4Seq a4_seq(const Kv4AttnArgs& a, int b) {
     s.rows = a.offsets ? max(a.offsets[b + 1] - s.first, 0) : 1;      // rows * group: q would not fit the device from 2^31 on
     s.len = max(0, min(a.lens[b], a.max_pages * a.page));
     s.tiles = (int)a.by_pairs.div((uint32_t)(s.rows * a.group + a.pairs - 1));
-    s.units = max(1, (s.len + A4_UNIT - 1) / A4_UNIT);
-    if (a.window > 0) s.units = (int)min((int64_t)s.units, ((int64_t)a.window + a.pairs / a.group + A4_UNIT + 1) / A4_UNIT + 1);
+    s.units = max(1, (s.len + A4_KEYS - 1) / A4_KEYS);
+    if (a.window > 0) s.units = (int)min((int64_t)s.units, ((int64_t)a.window + a.pairs / a.group + A4_KEYS + 1) / A4_KEYS + 1);
     return s;
 }
-__device__ __forceinline__ int64_t a4_units(const Kv4AttnArgs& a, const A4Seq& s) { return (int64_t)s.tiles * a.KV * s.units; }
+__device__ __forceinline__ int64_t a4_units(const Kv4AttnArgs& a, const A4Seq& s) { return (int64_t)s.tiles * a.KV * (s.units + A4_ITEM); }
 
 // The keys that the pairs of one tile see, in units: the item's units are first .. first + units - 1, of which those from `end` on
 // (keys from key_end on) hold nothing.
@@ -154,28 +179,26 @@ __device__ __forceinline__ A4Range a4_range(const Kv4AttnArgs& a, const A4Seq& s
     const int last = min(s.rows - 1, (int)a.by_group.div((uint32_t)((tile + 1) * a.pairs - 1)));
     A4Range r;
     r.key_end = max(0, s.len - s.rows + last + 1);
-    r.first = max(0, (r.key_end + A4_UNIT - 1) / A4_UNIT - s.units);
+    r.first = max(0, (r.key_end + A4_KEYS - 1) / A4_KEYS - s.units);
     return r;
 }
 
 template <int HD, int KIND, int NT>
-__global__ void __launch_bounds__(A4_THREADS, A4_BLOCKS) attn_kv4_kernel(const __grid_constant__ Kv4AttnArgs a) {
+__global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(const __grid_constant__ Kv4AttnArgs a) {
     using ST = A4Stage<HD, KIND>;
-    constexpr int NB = ST::NB;
+    constexpr int NB = ST::NB, STAGES = a4_stages(NT), RING = STAGES * ST::BYTES;
     constexpr uint32_t LOW = 0x000F000Fu, UP = 0x00F000F0u;      // code * 2^-24, code * 2^-20
     constexpr uint32_t LESS_8 = 0x80088008u, LESS_8_UP = 0x80808080u;        // -8 of each
     constexpr float ROUND = 12582912.0f;                         // 1.5 * 2^23
     extern __shared__ __align__(128) uint8_t a4_ring[];
-    __shared__ int64_t s_sum[A4_WARPS], s_rest;
-    __shared__ int s_b;
-    __shared__ float s_ml[A4_WARPS][4 * NT][2];
+    __shared__ int64_t s_sum[A4_WARPS], s_from[A4_THREADS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     asm volatile("griddepcontrol.launch_dependents;");
 
-    // ---- this block's share of the units ----
-    const int each = (a.batch + A4_THREADS - 1) / A4_THREADS, b0 = threadIdx.x * each;
+    // ---- this worker's share of the units ----
+    const int each = (a.batch + A4_THREADS - 1) / A4_THREADS;
     int64_t mine = 0;
-    for (int b = b0; b < min(a.batch, b0 + each); ++b) mine += a4_units(a, a4_seq(a, b));
+    for (int i = threadIdx.x * each; i < min(a.batch, (int)(threadIdx.x + 1) * each); ++i) mine += a4_units(a, a4_seq(a, i));
     int64_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -190,90 +213,115 @@ __global__ void __launch_bounds__(A4_THREADS, A4_BLOCKS) attn_kv4_kernel(const _
         if (w < warp) upto += s_sum[w];
         all += s_sum[w];
     }
-    const int64_t per = (all + gridDim.x - 1) / gridDim.x;
-    int64_t u = (int64_t)blockIdx.x * per;
-    const int64_t u_end = min(all, u + per);
-    if (threadIdx.x == 0) a.item[blockIdx.x] = make_int4(0, 0, 0, 0);
-    if (u >= u_end) return;
-    if (upto - mine <= u && u < upto) {
-        int64_t rest = u - (upto - mine);
-        int b = b0;
-        for (;; ++b) {
-            const int64_t n = a4_units(a, a4_seq(a, b));
-            if (rest < n) break;
-            rest -= n;
-        }
-        s_b = b;
-        s_rest = rest;
-    }
+    s_from[threadIdx.x] = upto - mine;
     __syncthreads();
-    int b = s_b;
-    int64_t rest = s_rest;
+    // the block's workers lie far apart, so that few of them still reach every SM
+    const int side = warp % a.across, worker = warp / a.across * gridDim.x + blockIdx.x, workers = A4_WARPS / a.across * gridDim.x;
+    const int64_t per = max((int64_t)A4_LEAST, (all + workers - 1) / workers);
+    int64_t u = worker * per;
+    const int64_t u_end = min(all, u + per);
+    if (lane == 0 && side == 0) a.item[worker].more = 0;
+    if (u >= u_end) return;
+    int b = -1;                                                  // the last thread whose sequences begin at u or before
+#pragma unroll
+    for (int i = 0; i < A4_WARPS; ++i) b += __popc(__ballot_sync(0xffffffffu, s_from[32 * i + lane] <= u));
+    int64_t rest = u - s_from[b];
+    b *= each;
     A4Seq seq = a4_seq(a, b);
+    while (rest >= a4_units(a, seq)) {
+        rest -= a4_units(a, seq);
+        seq = a4_seq(a, ++b);
+    }
 
     const bool wide = a.page % A4_KEYS == 0;                     // a warp's keys lie in one page
-    const int side = warp % a.across, step0 = warp / a.across, step = A4_WARPS / a.across * A4_KEYS;
-    uint8_t* ring = a4_ring + warp * ST::RING;
+    constexpr int step = A4_KEYS;
+    uint8_t* ring = a4_ring + warp * RING;
     const uint32_t ring_at = a4_smem(ring);
 
     while (true) {
-        const int64_t item = rest / seq.units;
-        const int i0 = (int)(rest - item * seq.units), i1 = (int)min((int64_t)seq.units, i0 + (u_end - u));
+        const int weight = seq.units + A4_ITEM;
+        const int64_t item = rest / weight;
+        const int w0 = (int)(rest - item * weight), w1 = (int)min((int64_t)weight, w0 + (u_end - u));
+        u += w1 - w0;
+        rest += w1 - w0;
+        const int i0 = max(0, w0 - A4_ITEM), i1 = max(0, w1 - A4_ITEM);
+        if (i0 == i1) break;                                     // the share ends before the item's first unit
         const int kv = (int)(item / seq.tiles), tile = (int)(item - (int64_t)kv * seq.tiles);
         const A4Range range = a4_range(a, seq, tile);
-        const int kbeg = (range.first + i0) * A4_UNIT, kend = (int)min((int64_t)range.key_end, ((int64_t)range.first + i1) * A4_UNIT);
+        const int kbeg = (range.first + i0) * A4_KEYS, kend = (int)min((int64_t)range.key_end, ((int64_t)range.first + i1) * A4_KEYS);
         const int32_t* table = a.table + (int64_t)b * a.max_pages;
         const int pair0 = tile * a.pairs + side * 4 * NT, npairs = seq.rows * a.group;
 
         // ---- one tile of 32 keys into stage s ----
-        auto page_of = [&](int k) { return k < kend ? table[a.by_page.div(wide ? k : min(k + lane, kend - 1))] : -1; };
-        auto issue = [&](int s, int k, int id) {
-            constexpr int CH = ST::ROW / 16, PER = 32 / CH;      // 16-byte pieces of a row, keys per round
-            const uint32_t dst = ring_at + s * ST::BYTES;
-            const bool there = (uint32_t)id < (uint32_t)a.num_pages;
-            const int key = min(k + (wide ? 0 : lane), kend - 1);
-            const int off = key - (int)a.by_page.div(key) * a.page;
-            const int64_t at = (int64_t)(there ? id : 0) * a.part.bytes;           // of the page
-            const int64_t row = (int64_t)kv * a.page + off;                              // of the tile's first key, or the lane's
+        // K rows stand in the order in which the fragments take them, V rows as they come, the pieces of every other pair of rows swapped
+        // so that four rows one apart miss each other's banks
+        constexpr int CH = ST::ROW / 16, PER = 32 / CH;          // 16-byte pieces of a row, keys per round
+        const int lkey = lane / CH, lpiece = lane % CH * 16;
+        const uint32_t kdst = ring_at + ((lkey & 8) + 2 * (lkey & 3) + ((lkey >> 2) & 1)) * ST::ROW + lpiece;
+        const uint32_t vdst = ring_at + ST::V + lkey * ST::ROW + (HD == 128 ? lpiece ^ ((lkey & 2) * 16) : lpiece);
+        const uint32_t sdst = ring_at + ST::KS + lane * ST::SROW;
+        struct Place {
+            int id, off;                                         // page and token in it: of the tile's first key, or (not wide) of the lane's
+        };
+        auto place = [&](int k) {
+            Place pl{-1, 0};
+            if (k < kend) {
+                const int key = wide ? k : min(k + lane, kend - 1), p = (int)a.by_page.div(key);
+                pl.id = table[p];
+                pl.off = key - p * a.page;
+            }
+            return pl;
+        };
+        auto issue = [&](int s, int k, Place pl) {
+            const uint32_t so = s * ST::BYTES;
+            const bool there = (uint32_t)pl.id < (uint32_t)a.num_pages;
+            const uint8_t* at = a.pages + (int64_t)(there ? pl.id : 0) * a.part.bytes;
+            const int64_t row = (int64_t)kv * a.page + pl.off;
+            if (wide && there && k + A4_KEYS <= kend) {
+                const uint8_t* p = at + row * ST::ROW + lkey * ST::ROW + lpiece;
+                const uint8_t* ps = at + a.part.k_scale + (row + lane) * ST::SROW;
+                const int64_t v_code = a.part.v_code;
+#pragma unroll
+                for (int i = 0; i < A4_KEYS / PER; ++i) {
+                    a4_copy<16>(kdst + so + i * PER * ST::ROW, p + i * PER * ST::ROW);
+                    a4_copy<16>(vdst + so + i * PER * ST::ROW, p + v_code + i * PER * ST::ROW);
+                }
+                a4_copy<ST::SROW>(sdst + so, ps);
+                a4_copy<ST::SROW>(sdst + so + (ST::VS - ST::KS), ps + v_code);     // the V parts follow the K parts in the same order
+                return;
+            }
 #pragma unroll
             for (int i = 0; i < A4_KEYS / PER; ++i) {
-                const int key_of = i * PER + lane / CH;
-                int64_t src;
-                bool ok = k + key_of < kend;
-                if (wide) {
-                    src = at + (row + key_of) * ST::ROW;
-                    ok = ok && there;
-                } else {
-                    src = __shfl_sync(0xffffffffu, at + row * ST::ROW, key_of);
-                    ok = __shfl_sync(0xffffffffu, there, key_of) && ok;
+                const int key_of = i * PER + lkey;
+                const uint8_t* p = at + (row + (wide ? key_of : 0)) * ST::ROW;
+                bool ok = there;
+                if (!wide) {
+                    p = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(p), key_of));
+                    ok = __shfl_sync(0xffffffffu, there, key_of);
                 }
-                if (!ok) src = 0;
-                const uint8_t* p = a.pages + src + lane % CH * 16;
-                // K rows in the order in which the fragments take them, V rows as they come, their pieces swapped so that four rows
-                // apart by one miss each other's banks
-                const int kr = (key_of & 24) + 2 * (key_of & 3) + ((key_of >> 2) & 1);
-                const int vc = HD == 128 ? lane % CH ^ (key_of & 2) : lane % CH;
-                a4_copy<16>(dst + kr * ST::ROW + lane % CH * 16, p, ok);
-                a4_copy<16>(dst + ST::V + key_of * ST::ROW + vc * 16, p + a.part.v_code, ok);
+                ok = ok && k + key_of < kend;
+                p = ok ? p + lpiece : a.pages;
+                a4_copy<16>(kdst + so + i * PER * ST::ROW, p, ok);
+                a4_copy<16>(vdst + so + i * PER * ST::ROW, p + a.part.v_code, ok);
             }
             const bool ok = k + lane < kend && there;
-            const uint8_t* p = a.pages + (ok ? at + (row + (wide ? lane : 0)) * ST::SROW : 0);
-            a4_copy<ST::SROW>(dst + ST::KS + lane * ST::SROW, p + a.part.k_scale, ok);
-            a4_copy<ST::SROW>(dst + ST::VS + lane * ST::SROW, p + a.part.v_scale, ok);
+            const uint8_t* p = ok ? at + (row + (wide ? lane : 0)) * ST::SROW : a.pages;
+            a4_copy<ST::SROW>(sdst + so, p + a.part.k_scale, ok);
+            a4_copy<ST::SROW>(sdst + so + (ST::VS - ST::KS), p + a.part.v_scale, ok);
         };
         auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
 
-        int k = kbeg + step0 * A4_KEYS;
+        int k = kbeg;
 #pragma unroll
-        for (int s = 0; s < A4_STAGES - 1; ++s) {
-            if (k + s * step < kend) issue(s, k + s * step, page_of(k + s * step));
+        for (int s = 0; s < STAGES - 1; ++s) {
+            if (k + s * step < kend) issue(s, k + s * step, place(k + s * step));
             commit();
         }
-        int next_id = page_of(k + (A4_STAGES - 1) * step);
+        Place next = place(k + (STAGES - 1) * step);
 
         // ---- queries: parts of q 2^e as B fragments, sums of each block ----
         uint32_t qf[NT][NB][2][2];
-        float qsum[NT][NB], unit[NT];
+        float qsum[NT][NB], less[NT][NB][2], unit[NT];            // kind 1: sums of the blocks; kind 0: -8 times those of the parts
         int lim[NT], from[NT];
         int all_see = 0x7fffffff, none_before = 0;
 #pragma unroll
@@ -302,15 +350,29 @@ __global__ void __launch_bounds__(A4_THREADS, A4_BLOCKS) attn_kv4_kernel(const _
             const float back = __uint_as_float((uint32_t)(e == 255 ? 254 : e) << 23) * 16384.0f;     // 2^24 / mul
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
-                float sum = ((x[n][0] + x[n][1]) + (x[n][2] + x[n][3])) + ((x[n][4] + x[n][5]) + (x[n][6] + x[n][7]));
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                qsum[j][n] = __shfl_sync(0xffffffffu, sum * mul * 0x1p-24f, 8 * t);
+                float sum = 0.0f, rest = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     // nibble i of two words, elements i and 4 + i; an odd nibble's codes come 16 times too large
                     const float f = i & 1 ? 0.0625f : 1.0f, u0 = x[n][i] * mul, u1 = x[n][4 + i] * mul, h0 = rintf(u0), h1 = rintf(u1);
-                    qf[j][n][i >> 1][i & 1] = g & 1 ? a4_pack((u0 - h0) * f, (u1 - h1) * f) : a4_pack(h0 * f, h1 * f);
+                    const uint32_t low = a4_pack((u0 - h0) * f, (u1 - h1) * f);
+                    qf[j][n][i >> 1][i & 1] = g & 1 ? low : a4_pack(h0 * f, h1 * f);
+                    if (KIND == 0) {
+                        const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&low));
+                        sum += h0 + h1;
+                        rest += (r.x + r.y) * (i & 1 ? 16.0f : 1.0f);
+                    } else {
+                        sum += u0 + u1;
+                    }
+                }
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                if (KIND == 1) qsum[j][n] = __shfl_sync(0xffffffffu, sum * 0x1p-24f, 8 * t);
+                if (KIND == 0) {
+                    rest += __shfl_xor_sync(0xffffffffu, rest, 1);
+                    rest += __shfl_xor_sync(0xffffffffu, rest, 2);
+                    less[j][n][0] = __shfl_sync(0xffffffffu, sum * -0x1p-21f, 8 * t);
+                    less[j][n][1] = __shfl_sync(0xffffffffu, rest * -0x1p-21f, 8 * t);
                 }
             }
             unit[j] = __shfl_sync(0xffffffffu, back, 8 * t) * (a.scale * 1.4426950408889634f);       // to powers of two
@@ -337,14 +399,14 @@ __global__ void __launch_bounds__(A4_THREADS, A4_BLOCKS) attn_kv4_kernel(const _
         }
         const int kk = (g >> 1) + 4 * (g & 1);                    // key (of 8) that fragment row g is
 
-        for (int s = 0; k < kend; k += step, s = s + 1 == A4_STAGES ? 0 : s + 1) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(A4_STAGES - 2) : "memory");
+        for (int s = 0; k < kend; k += step, s = s + 1 == STAGES ? 0 : s + 1) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
             __syncwarp();                                         // this tile is here, and the one before it is read
             {
-                const int ahead = k + (A4_STAGES - 1) * step;
-                if (ahead < kend) issue(s == 0 ? A4_STAGES - 1 : s - 1, ahead, next_id);
+                const int ahead = k + (STAGES - 1) * step;
+                if (ahead < kend) issue(s == 0 ? STAGES - 1 : s - 1, ahead, next);
                 commit();
-                next_id = page_of(ahead + step);
+                next = place(ahead + step);
             }
             const uint8_t* st = ring + s * ST::BYTES;
 
@@ -381,10 +443,15 @@ __global__ void __launch_bounds__(A4_THREADS, A4_BLOCKS) attn_kv4_kernel(const _
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
                         float c[4];
-                        a4_mma0(c, w[0][n] & LOW, w[1][n] & LOW, w[0][n] & UP, w[1][n] & UP, qf[j][n][0][0], qf[j][n][0][1]);
+                        if (KIND == 0) a4_mma_from(c, less[j][n][0], less[j][n][1], w[0][n] & LOW, w[1][n] & LOW, w[0][n] & UP, w[1][n] & UP, qf[j][n][0][0], qf[j][n][0][1]);
+                        else a4_mma0(c, w[0][n] & LOW, w[1][n] & LOW, w[0][n] & UP, w[1][n] & UP, qf[j][n][0][0], qf[j][n][0][1]);
                         a4_mma(c, s0 & LOW, s1 & LOW, s0 & UP, s1 & UP, qf[j][n][1][0], qf[j][n][1][1]);
-                        x[j][2 * h] = fmaf(m0, qsum[j][n], fmaf(d0, c[0] + c[1], x[j][2 * h]));
-                        x[j][2 * h + 1] = fmaf(m1, qsum[j][n], fmaf(d1, c[2] + c[3], x[j][2 * h + 1]));
+                        x[j][2 * h] = fmaf(d0, c[0] + c[1], x[j][2 * h]);
+                        x[j][2 * h + 1] = fmaf(d1, c[2] + c[3], x[j][2 * h + 1]);
+                        if (KIND == 1) {
+                            x[j][2 * h] = fmaf(m0, qsum[j][n], x[j][2 * h]);
+                            x[j][2 * h + 1] = fmaf(m1, qsum[j][n], x[j][2 * h + 1]);
+                        }
                     }
                 }
             }
@@ -430,13 +497,10 @@ __global__ void __launch_bounds__(A4_THREADS, A4_BLOCKS) attn_kv4_kernel(const _
             for (int i = 0; i < 4; ++i) {
                 sv[i].load(st + ST::VS + (8 * i + kk) * ST::SROW);
 #pragma unroll
-                for (int n = 0; n < A4Scales<KIND, NB>::WORDS; ++n) {
-                    const uint32_t mag = sv[i].w[n] & 0x7FFF7FFFu;
-                    top_d = KIND == 1 ? max(top_d, mag & 0xFFFFu) : __vmaxu2(top_d, mag);
-                }
+                for (int n = 0; n < A4Scales<KIND, NB>::WORDS; ++n) top_d = __vmaxu2(top_d, sv[i].w[n]);      // kind 1: m beside it, unused
             }
             if (KIND == 0) top_d = max(top_d & 0xFFFFu, top_d >> 16);
-            const float largest = half_bits_to_float((uint16_t)__reduce_max_sync(0xffffffffu, top_d));
+            const float largest = half_bits_to_float((uint16_t)(__reduce_max_sync(0xffffffffu, top_d & 0x7FFFu)));
             float pg[NT][4], shrink[NT];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
@@ -503,98 +567,109 @@ __global__ void __launch_bounds__(A4_THREADS, A4_BLOCKS) attn_kv4_kernel(const _
                 }
             }
         }
-        // ---- the lanes' sums, then the warps' ----
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        __syncthreads();                                          // the rings become the warps' results
-        float* res = reinterpret_cast<float*>(a4_ring);           // [warp][pair][HD]
+        // ---- the lanes' sums ----
+        const bool whole = i0 == 0 && i1 == seq.units;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
 #pragma unroll
             for (int sh = 4; sh < 32; sh <<= 1) {
                 l[j] += __shfl_xor_sync(0xffffffffu, l[j], sh);
 #pragma unroll
-                for (int n = 0; n < NB; ++n) bias[j][n] += __shfl_xor_sync(0xffffffffu, bias[j][n], sh);
+                for (int n = 0; n < NB; ++n)
+                    if (KIND == 1) bias[j][n] += __shfl_xor_sync(0xffffffffu, bias[j][n], sh);
             }
+            const int p = pair0 + 4 * j + t;
+            if (p >= npairs) continue;
+            const int row = (int)a.by_group.div(p);
+            float* piece = a.piece + ((int64_t)(2 * worker + (i0 == 0)) * a.pairs + side * 4 * NT + 4 * j + t) * (HD + 4);
+            float* dst = whole ? a.out + (int64_t)(seq.first + row) * a.os + ((int64_t)kv * a.group + (p - row * a.group)) * HD : piece;
+            const float mul = !whole ? 1.0f : l[j] == 0.0f ? 0.0f : 1.0f / l[j];
 #pragma unroll
             for (int n = 0; n < NB; ++n)
-                *reinterpret_cast<float4*>(res + (warp * 4 * NT + 4 * j + t) * HD + 32 * n + 4 * g) =
-                    make_float4(o[j][2 * n][0] + bias[j][n], fmaf(o[j][2 * n][1], 0.0625f, bias[j][n]), o[j][2 * n + 1][0] + bias[j][n],
-                                fmaf(o[j][2 * n + 1][1], 0.0625f, bias[j][n]));
-            if (g == 0) {
-                s_ml[warp][4 * j + t][0] = m[j];
-                s_ml[warp][4 * j + t][1] = l[j];
+                *reinterpret_cast<float4*>(dst + 32 * n + 4 * g) =
+                    make_float4((o[j][2 * n][0] + bias[j][n]) * mul, fmaf(o[j][2 * n][1], 0.0625f, bias[j][n]) * mul,
+                                (o[j][2 * n + 1][0] + bias[j][n]) * mul, fmaf(o[j][2 * n + 1][1], 0.0625f, bias[j][n]) * mul);
+            if (!whole && g == 0) {
+                piece[HD] = m[j];
+                piece[HD + 1] = l[j];
             }
         }
-        __syncthreads();
-        const bool whole = i0 == 0 && i1 == seq.units;
-        const int slot = 2 * blockIdx.x + (i0 == 0);
-        const int npr = min(a.pairs, npairs - tile * a.pairs);
-        for (int i = threadIdx.x; i < npr * (HD / 4); i += A4_THREADS) {
-            const int p = i / (HD / 4), c = i % (HD / 4) * 4, sd = p / (4 * NT), pp = p % (4 * NT);
-            float mm = -INFINITY, ll = 0.0f;
-            for (int w = sd; w < A4_WARPS; w += a.across) mm = fmaxf(mm, s_ml[w][pp][0]);
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int w = sd; w < A4_WARPS; w += a.across) {
-                const float lw = s_ml[w][pp][1];
-                const float f = s_ml[w][pp][0] == -INFINITY && lw == 0.0f ? 0.0f : a4_exp2(s_ml[w][pp][0] - mm);
-                const float4 v = *reinterpret_cast<const float4*>(res + (w * 4 * NT + pp) * HD + c);
-                ll += lw * f;
-                acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
-            }
-            if (whole) {
-                const int of = tile * a.pairs + p, row = (int)a.by_group.div(of);
-                const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-                float* dst = a.out + (int64_t)(seq.first + row) * a.os + ((int64_t)kv * a.group + (of - row * a.group)) * HD + c;
-                *reinterpret_cast<float4*>(dst) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-            } else {
-                float* dst = a.piece + ((int64_t)slot * a.pairs + p) * (HD + 4);
-                *reinterpret_cast<float4*>(dst + c) = acc;
-                if (c == 0) { dst[HD] = mm; dst[HD + 1] = ll; }
-            }
-        }
-        if (i0 == 0 && !whole && threadIdx.x == 0) {
-            const int64_t more = seq.units - i1;                  // units of this item in the blocks that follow
-            a.item[blockIdx.x] = make_int4((int)((more + per - 1) / per), b, tile, kv);
-        }
-        u += i1 - i0;
-        if (u >= u_end) return;
-        rest += i1 - i0;
+        if (i0 == 0 && !whole && lane == 0 && side == 0)         // units of this item with the workers that follow
+            a.item[worker] = A4Item{(int)((seq.units - i1 + per - 1) / per), seq.first, tile * a.pairs, min(a.pairs, npairs - tile * a.pairs), kv, {0, 0, 0}};
+        if (u >= u_end) break;
         if (rest >= a4_units(a, seq)) {
             rest = 0;
             do seq = a4_seq(a, ++b); while (seq.rows == 0);       // there is one: units are left
         }
-        __syncthreads();                                          // the results are read, the rings may fill again
+        __syncwarp();                                             // the ring is read
     }
 }
 
-// Items that a block began and others went on with: one block each.
+// Items that a worker began and others went on with: one block each (two where the pairs are 16, four where they are 32), a thread per four
+// dims of a pair, eight pieces at a time; what threads that leaves take every other piece.
+constexpr int A4_JOIN = 256;
+
 template <int HD>
-__global__ void __launch_bounds__(A4_THREADS) attn_kv4_join_kernel(const __grid_constant__ Kv4AttnArgs a) {
+__global__ void __launch_bounds__(A4_JOIN) attn_kv4_join_kernel(const __grid_constant__ Kv4AttnArgs a) {
+    constexpr int AT_ONCE = 8;
+    __shared__ float4 s_o[A4_JOIN];
+    __shared__ float2 s_ml[A4_JOIN];
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int4 it = __ldcg(a.item + blockIdx.x);
-    if (it.x == 0) return;
-    const A4Seq seq = a4_seq(a, it.y);
-    const int first = it.z * a.pairs, npr = min(a.pairs, seq.rows * a.group - first);
-    // piece i: the block's own second slot, then the first slots of those behind it
-    auto piece = [&](int i, int p) { return a.piece + ((int64_t)(2 * (blockIdx.x + i) + (i == 0)) * a.pairs + p) * (HD + 4); };
-    for (int i = blockIdx.y * A4_THREADS + threadIdx.x; i < npr * (HD / 4); i += gridDim.y * A4_THREADS) {
-        const int p = i / (HD / 4), c = i % (HD / 4) * 4;
-        float mm = -INFINITY, ll = 0.0f;
-        for (int n = 0; n <= it.x; ++n) mm = fmaxf(mm, __ldcg(piece(n, p) + HD));
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int n = 0; n <= it.x; ++n) {
-            const float* s = piece(n, p);
-            const float ln = __ldcg(s + HD + 1), mn = __ldcg(s + HD);
-            const float f = mn == -INFINITY && ln == 0.0f ? 0.0f : a4_exp2(mn - mm);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(s + c));
-            ll += ln * f;
-            acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+    const A4Item it = a.item[blockIdx.x];
+    if (it.more == 0) return;
+    const int columns = min(a.pairs * (HD / 4), A4_JOIN), groups = A4_JOIN / columns, group = threadIdx.x / columns;
+    const int col = blockIdx.y * A4_JOIN + threadIdx.x % columns, p = col / (HD / 4), c = col % (HD / 4) * 4;
+    // piece i: the worker's own second slot, then the first slots of those behind it
+    const float* mine = a.piece + ((int64_t)(2 * blockIdx.x) * a.pairs + p) * (HD + 4);
+    float mm = -INFINITY, ll = 0.0f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = group; i0 <= it.more; i0 += AT_ONCE * groups) {
+        float2 ml[AT_ONCE];
+        float4 v[AT_ONCE];
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) {
+            const int i = i0 + k * groups;
+            ml[k] = make_float2(-INFINITY, 0.0f);
+            v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (i <= it.more) {
+                const float* s = mine + (int64_t)(2 * i + (i == 0)) * a.pairs * (HD + 4);
+                ml[k] = __ldcg(reinterpret_cast<const float2*>(s + HD));
+                v[k] = __ldcg(reinterpret_cast<const float4*>(s + c));
+            }
         }
-        const int row = (int)a.by_group.div(first + p);
-        const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-        float* dst = a.out + (int64_t)(seq.first + row) * a.os + ((int64_t)it.w * a.group + (first + p - row * a.group)) * HD + c;
-        *reinterpret_cast<float4*>(dst) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+        float top = mm;
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) top = fmaxf(top, ml[k].x);
+        const float base = top == -INFINITY ? 0.0f : top, old = a4_exp2(mm - base);
+        ll *= old;
+        acc.x *= old; acc.y *= old; acc.z *= old; acc.w *= old;
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) {
+            const float f = a4_exp2(ml[k].x - base);
+            ll = fmaf(ml[k].y, f, ll);
+            acc.x = fmaf(v[k].x, f, acc.x); acc.y = fmaf(v[k].y, f, acc.y); acc.z = fmaf(v[k].z, f, acc.z); acc.w = fmaf(v[k].w, f, acc.w);
+        }
+        mm = top;
     }
+    if (groups > 1) {
+        s_o[threadIdx.x] = acc;
+        s_ml[threadIdx.x] = make_float2(mm, ll);
+        __syncthreads();
+        if (group != 0) return;
+        for (int i = 1; i < groups; ++i) {
+            const float2 ml = s_ml[i * columns + threadIdx.x];
+            const float4 v = s_o[i * columns + threadIdx.x];
+            const float top = fmaxf(mm, ml.x), base = top == -INFINITY ? 0.0f : top, f0 = a4_exp2(mm - base), f1 = a4_exp2(ml.x - base);
+            ll = ll * f0 + ml.y * f1;
+            acc.x = acc.x * f0 + v.x * f1; acc.y = acc.y * f0 + v.y * f1; acc.z = acc.z * f0 + v.z * f1; acc.w = acc.w * f0 + v.w * f1;
+            mm = top;
+        }
+    }
+    if (p >= it.live) return;
+    const int row = (int)a.by_group.div(it.pair + p);
+    const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+    float* dst = a.out + (int64_t)(it.first + row) * a.os + ((int64_t)it.kv * a.group + (it.pair + p - row * a.group)) * HD + c;
+    *reinterpret_cast<float4*>(dst) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
 }
 
 // Pairs of a warp (4 or 8) and warps that take different pairs, from the most pairs that a sequence has for a KV head.
@@ -602,12 +677,12 @@ static void a4_shape(int64_t most, int& nt, int& across) {
     nt = most <= 4 ? 1 : 2;
     across = most <= 8 ? 1 : most <= 16 ? 2 : 4;
 }
-static int a4_blocks() { return A4_BLOCKS * num_sms(); }
+static int a4_blocks(int nt) { return a4_resident(nt) * num_sms(); }
 
 template <int HD, int KIND, int NT>
 static int launch_a4(const Kv4AttnArgs& a, int blocks) {
     auto kern = attn_kv4_kernel<HD, KIND, NT>;
-    constexpr int smem = A4_WARPS * A4Stage<HD, KIND>::RING;
+    constexpr int smem = A4_WARPS * a4_stages(NT) * A4Stage<HD, KIND>::BYTES;
     if (smem > 48 * 1024) B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     return launch_serve("attn_kv4_kernel", kern, dim3(blocks), dim3(A4_THREADS), smem, 1, false, a);
 }
@@ -625,7 +700,7 @@ int b200_attention_paged_kv4_workspace(int H, int KV, int hd, int max_rows, size
     B200_REQUIRE(H >= 1 && H % KV == 0 && max_rows >= 1, "attention_paged_kv4_workspace: H must be a positive multiple of KV, max_rows positive");
     int nt, across;
     a4_shape((int64_t)max_rows * (H / KV), nt, across);
-    *bytes = (size_t)a4_blocks() * (sizeof(int4) + (size_t)2 * 4 * nt * across * (hd + 4) * sizeof(float));
+    *bytes = (size_t)a4_blocks(nt) * (A4_WARPS / across) * (sizeof(A4Item) + (size_t)2 * 4 * nt * across * (hd + 4) * sizeof(float));
     return B200_OK;
 }
 
@@ -649,10 +724,10 @@ int b200_attention_paged_kv4(const float* q, int64_t q_stride, const int32_t* ro
     B200_REQUIRE(workspace_bytes >= need, "%s: the workspace has %zu bytes of %zu", who, workspace_bytes, need);
     int nt, across;
     a4_shape((int64_t)max_rows * (H / KV), nt, across);
-    const int blocks = a4_blocks();
+    const int blocks = a4_blocks(nt), workers = blocks * (A4_WARPS / across);
     Kv4AttnArgs a{q, q_stride, row_offsets, static_cast<const uint8_t*>(pages), num_pages, page_table, seq_lens, out, out_stride, batch,
                   max_pages, page, H, KV, H / KV, FastDiv(page), FastDiv(H / KV), FastDiv(4 * nt * across), Kv4Page(page, KV, hd, kind), scale, window, across, 4 * nt * across,
-                  reinterpret_cast<float*>(static_cast<int4*>(workspace) + blocks), static_cast<int4*>(workspace)};
+                  reinterpret_cast<float*>(static_cast<A4Item*>(workspace) + workers), static_cast<A4Item*>(workspace)};
     if (hd == 64)
         rc = kind == 1 ? (nt == 1 ? launch_a4<64, 1, 1>(a, blocks) : launch_a4<64, 1, 2>(a, blocks))
                        : (nt == 1 ? launch_a4<64, 0, 1>(a, blocks) : launch_a4<64, 0, 2>(a, blocks));
@@ -660,9 +735,9 @@ int b200_attention_paged_kv4(const float* q, int64_t q_stride, const int32_t* ro
         rc = kind == 1 ? (nt == 1 ? launch_a4<128, 1, 1>(a, blocks) : launch_a4<128, 1, 2>(a, blocks))
                        : (nt == 1 ? launch_a4<128, 0, 1>(a, blocks) : launch_a4<128, 0, 2>(a, blocks));
     if (rc) return rc;
-    const dim3 grid(blocks, std::max(1, a.pairs * (hd / 4) / A4_THREADS));
-    return hd == 64 ? launch_serve("attn_kv4_join_kernel", attn_kv4_join_kernel<64>, grid, dim3(A4_THREADS), 0, 1, true, a)
-                    : launch_serve("attn_kv4_join_kernel", attn_kv4_join_kernel<128>, grid, dim3(A4_THREADS), 0, 1, true, a);
+    const dim3 grid(workers, std::max(1, a.pairs * (hd / 4) / A4_JOIN));
+    return hd == 64 ? launch_serve("attn_kv4_join_kernel", attn_kv4_join_kernel<64>, grid, dim3(A4_JOIN), 0, 1, true, a)
+                    : launch_serve("attn_kv4_join_kernel", attn_kv4_join_kernel<128>, grid, dim3(A4_JOIN), 0, 1, true, a);
 }
 
 }  // extern "C"
