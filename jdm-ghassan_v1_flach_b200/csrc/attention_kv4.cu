@@ -19,11 +19,12 @@
 // What bounds it: for single tokens the cache, 2 KV (hd/2 + 4 hd/32) bytes a token once (kind 1), with about 600 instructions of a
 // warp per 32 keys behind it - two thirds of what an SM can issue in the time the bytes take; for many rows the instructions.
 //
-// The split.  The lengths are on the device, so the grid is fixed (three blocks on every SM) and every block takes an equal share of all
-// (sequence, tile of pairs, KV head, 128 keys) units laid end to end, found from a prefix sum over the batch that
+// The split.  The lengths are on the device, so the grid is fixed and every warp takes an equal share of all (sequence, KV head, tile of
+// 4 or 8 pairs, 32 keys) units laid end to end, with what an item's set-up costs counted in, found from a prefix sum over the batch that
 // every block makes by itself.  What a share cuts off an item's ends goes to the workspace and is joined by a second, small kernel.
-// A warp takes 32 keys at a time for 4 or 8 pairs, from a ring of its own in shared memory that cp.async fills two tiles ahead;
-// where a sequence has more pairs the block's warps take different pairs instead of different keys.
+// (Shares of whole blocks, their warps joined in shared memory: 74 us where this takes 64.  Warps of a block on different pairs of the
+// same keys: idle ones where the pairs are no multiple, 149 us on the drafts below.)  Keys come through a ring of each warp's own in
+// shared memory that cp.async fills two tiles ahead.
 #include <algorithm>
 
 #include "serve.cuh"
@@ -45,6 +46,8 @@ constexpr int A4_KEYS = 32;                      // keys of a warp's step
 #endif
 // Stages of a warp's ring and blocks of an SM, by the warp's tiles of four pairs.
 __host__ __device__ constexpr int a4_stages(int nt) { return nt == 1 ? A4_S1 : A4_S2; }
+// A warp's query fragments where they stay in shared memory: 32 registers that two tiles of pairs have more use for.
+__host__ __device__ constexpr int a4_query_bytes(int hd, int nt) { return nt > 1 ? nt * (hd / 32) * 32 * 16 : 0; }
 __host__ __device__ constexpr int a4_resident(int nt) { return nt == 1 ? A4_B1 : A4_B2; }
 
 struct Kv4AttnArgs {
@@ -62,8 +65,7 @@ struct Kv4AttnArgs {
     Kv4Page part;
     float scale;
     int window;
-    int across;                                  // warps of a worker: they take different pairs
-    int pairs;                                   // of a worker
+    int pairs;                                   // of a tile
     float* piece;                                // [2 * workers][pairs][hd + 4]: o, m, l of cut items
     struct A4Item* item;                         // [workers]
 };
@@ -186,7 +188,7 @@ __device__ __forceinline__ A4Range a4_range(const Kv4AttnArgs& a, const A4Seq& s
 template <int HD, int KIND, int NT>
 __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(const __grid_constant__ Kv4AttnArgs a) {
     using ST = A4Stage<HD, KIND>;
-    constexpr int NB = ST::NB, STAGES = a4_stages(NT), RING = STAGES * ST::BYTES;
+    constexpr int NB = ST::NB, PAIRS = 4 * NT, STAGES = a4_stages(NT), RING = STAGES * ST::BYTES;
     constexpr uint32_t LOW = 0x000F000Fu, UP = 0x00F000F0u;      // code * 2^-24, code * 2^-20
     constexpr uint32_t LESS_8 = 0x80088008u, LESS_8_UP = 0x80808080u;        // -8 of each
     constexpr float ROUND = 12582912.0f;                         // 1.5 * 2^23
@@ -216,11 +218,11 @@ __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(c
     s_from[threadIdx.x] = upto - mine;
     __syncthreads();
     // the block's workers lie far apart, so that few of them still reach every SM
-    const int side = warp % a.across, worker = warp / a.across * gridDim.x + blockIdx.x, workers = A4_WARPS / a.across * gridDim.x;
+    const int worker = warp * gridDim.x + blockIdx.x, workers = A4_WARPS * gridDim.x;
     const int64_t per = max((int64_t)A4_LEAST, (all + workers - 1) / workers);
     int64_t u = worker * per;
     const int64_t u_end = min(all, u + per);
-    if (lane == 0 && side == 0) a.item[worker].more = 0;
+    if (lane == 0) a.item[worker].more = 0;
     if (u >= u_end) return;
     int b = -1;                                                  // the last thread whose sequences begin at u or before
 #pragma unroll
@@ -235,7 +237,9 @@ __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(c
 
     const bool wide = a.page % A4_KEYS == 0;                     // a warp's keys lie in one page
     constexpr int step = A4_KEYS;
+    constexpr bool Q_SHARED = NT > 1;
     uint8_t* ring = a4_ring + warp * RING;
+    uint4(*s_q)[32] = reinterpret_cast<uint4(*)[32]>(a4_ring + A4_WARPS * RING + warp * a4_query_bytes(HD, NT));
     const uint32_t ring_at = a4_smem(ring);
 
     while (true) {
@@ -250,7 +254,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(c
         const A4Range range = a4_range(a, seq, tile);
         const int kbeg = (range.first + i0) * A4_KEYS, kend = (int)min((int64_t)range.key_end, ((int64_t)range.first + i1) * A4_KEYS);
         const int32_t* table = a.table + (int64_t)b * a.max_pages;
-        const int pair0 = tile * a.pairs + side * 4 * NT, npairs = seq.rows * a.group;
+        const int pair0 = tile * PAIRS, npairs = seq.rows * a.group;
 
         // ---- one tile of 32 keys into stage s ----
         // K rows stand in the order in which the fragments take them, V rows as they come, the pieces of every other pair of rows swapped
@@ -320,7 +324,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(c
         Place next = place(k + (STAGES - 1) * step);
 
         // ---- queries: parts of q 2^e as B fragments, sums of each block ----
-        uint32_t qf[NT][NB][2][2];
+        uint32_t qf[NT][NB][2][2];                                // NT > 1: kept in shared memory
         float qsum[NT][NB], less[NT][NB][2], unit[NT];            // kind 1: sums of the blocks; kind 0: -8 times those of the parts
         int lim[NT], from[NT];
         int all_see = 0x7fffffff, none_before = 0;
@@ -374,6 +378,10 @@ __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(c
                     less[j][n][0] = __shfl_sync(0xffffffffu, sum * -0x1p-21f, 8 * t);
                     less[j][n][1] = __shfl_sync(0xffffffffu, rest * -0x1p-21f, 8 * t);
                 }
+            }
+            if (Q_SHARED) {
+#pragma unroll
+                for (int n = 0; n < NB; ++n) s_q[j * NB + n][lane] = make_uint4(qf[j][n][0][0], qf[j][n][0][1], qf[j][n][1][0], qf[j][n][1][1]);
             }
             unit[j] = __shfl_sync(0xffffffffu, back, 8 * t) * (a.scale * 1.4426950408889634f);       // to powers of two
             const int pt = pair0 + 4 * j + t;
@@ -443,9 +451,10 @@ __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(c
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
                         float c[4];
-                        if (KIND == 0) a4_mma_from(c, less[j][n][0], less[j][n][1], w[0][n] & LOW, w[1][n] & LOW, w[0][n] & UP, w[1][n] & UP, qf[j][n][0][0], qf[j][n][0][1]);
-                        else a4_mma0(c, w[0][n] & LOW, w[1][n] & LOW, w[0][n] & UP, w[1][n] & UP, qf[j][n][0][0], qf[j][n][0][1]);
-                        a4_mma(c, s0 & LOW, s1 & LOW, s0 & UP, s1 & UP, qf[j][n][1][0], qf[j][n][1][1]);
+                        const uint4 f = Q_SHARED ? s_q[j * NB + n][lane] : make_uint4(qf[j][n][0][0], qf[j][n][0][1], qf[j][n][1][0], qf[j][n][1][1]);
+                        if (KIND == 0) a4_mma_from(c, less[j][n][0], less[j][n][1], w[0][n] & LOW, w[1][n] & LOW, w[0][n] & UP, w[1][n] & UP, f.x, f.y);
+                        else a4_mma0(c, w[0][n] & LOW, w[1][n] & LOW, w[0][n] & UP, w[1][n] & UP, f.x, f.y);
+                        a4_mma(c, s0 & LOW, s1 & LOW, s0 & UP, s1 & UP, f.z, f.w);
                         x[j][2 * h] = fmaf(d0, c[0] + c[1], x[j][2 * h]);
                         x[j][2 * h + 1] = fmaf(d1, c[2] + c[3], x[j][2 * h + 1]);
                         if (KIND == 1) {
@@ -581,7 +590,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(c
             const int p = pair0 + 4 * j + t;
             if (p >= npairs) continue;
             const int row = (int)a.by_group.div(p);
-            float* piece = a.piece + ((int64_t)(2 * worker + (i0 == 0)) * a.pairs + side * 4 * NT + 4 * j + t) * (HD + 4);
+            float* piece = a.piece + ((int64_t)(2 * worker + (i0 == 0)) * PAIRS + 4 * j + t) * (HD + 4);
             float* dst = whole ? a.out + (int64_t)(seq.first + row) * a.os + ((int64_t)kv * a.group + (p - row * a.group)) * HD : piece;
             const float mul = !whole ? 1.0f : l[j] == 0.0f ? 0.0f : 1.0f / l[j];
 #pragma unroll
@@ -594,8 +603,8 @@ __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(c
                 piece[HD + 1] = l[j];
             }
         }
-        if (i0 == 0 && !whole && lane == 0 && side == 0)         // units of this item with the workers that follow
-            a.item[worker] = A4Item{(int)((seq.units - i1 + per - 1) / per), seq.first, tile * a.pairs, min(a.pairs, npairs - tile * a.pairs), kv, {0, 0, 0}};
+        if (i0 == 0 && !whole && lane == 0)         // units of this item with the workers that follow
+            a.item[worker] = A4Item{(int)((seq.units - i1 + per - 1) / per), seq.first, pair0, min(PAIRS, npairs - pair0), kv, {0, 0, 0}};
         if (u >= u_end) break;
         if (rest >= a4_units(a, seq)) {
             rest = 0;
@@ -605,8 +614,8 @@ __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(c
     }
 }
 
-// Items that a worker began and others went on with: one block each (two where the pairs are 16, four where they are 32), a thread per four
-// dims of a pair, eight pieces at a time; what threads that leaves take every other piece.
+// Items that a worker began and others went on with: one block each, a thread per four dims of a pair, eight pieces at a time; what threads
+// that leaves take every other piece.
 constexpr int A4_JOIN = 256;
 
 template <int HD>
@@ -617,8 +626,8 @@ __global__ void __launch_bounds__(A4_JOIN) attn_kv4_join_kernel(const __grid_con
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const A4Item it = a.item[blockIdx.x];
     if (it.more == 0) return;
-    const int columns = min(a.pairs * (HD / 4), A4_JOIN), groups = A4_JOIN / columns, group = threadIdx.x / columns;
-    const int col = blockIdx.y * A4_JOIN + threadIdx.x % columns, p = col / (HD / 4), c = col % (HD / 4) * 4;
+    const int columns = a.pairs * (HD / 4), groups = A4_JOIN / columns, group = threadIdx.x / columns;
+    const int col = threadIdx.x % columns, p = col / (HD / 4), c = col % (HD / 4) * 4;
     // piece i: the worker's own second slot, then the first slots of those behind it
     const float* mine = a.piece + ((int64_t)(2 * blockIdx.x) * a.pairs + p) * (HD + 4);
     float mm = -INFINITY, ll = 0.0f;
@@ -672,17 +681,14 @@ __global__ void __launch_bounds__(A4_JOIN) attn_kv4_join_kernel(const __grid_con
     *reinterpret_cast<float4*>(dst) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
 }
 
-// Pairs of a warp (4 or 8) and warps that take different pairs, from the most pairs that a sequence has for a KV head.
-static void a4_shape(int64_t most, int& nt, int& across) {
-    nt = most <= 4 ? 1 : 2;
-    across = most <= 8 ? 1 : most <= 16 ? 2 : 4;
-}
+// Tiles of four pairs that a warp takes at once, from the most pairs that a sequence has for a KV head.
+static int a4_tiles(int64_t most) { return most <= 4 ? 1 : 2; }
 static int a4_blocks(int nt) { return a4_resident(nt) * num_sms(); }
 
 template <int HD, int KIND, int NT>
 static int launch_a4(const Kv4AttnArgs& a, int blocks) {
     auto kern = attn_kv4_kernel<HD, KIND, NT>;
-    constexpr int smem = A4_WARPS * a4_stages(NT) * A4Stage<HD, KIND>::BYTES;
+    constexpr int smem = A4_WARPS * (a4_stages(NT) * A4Stage<HD, KIND>::BYTES + a4_query_bytes(HD, NT));
     if (smem > 48 * 1024) B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     return launch_serve("attn_kv4_kernel", kern, dim3(blocks), dim3(A4_THREADS), smem, 1, false, a);
 }
@@ -698,9 +704,8 @@ int b200_attention_paged_kv4_workspace(int H, int KV, int hd, int max_rows, size
     if (rc) return rc;
     B200_REQUIRE(bytes, "attention_paged_kv4_workspace: null pointer");
     B200_REQUIRE(H >= 1 && H % KV == 0 && max_rows >= 1, "attention_paged_kv4_workspace: H must be a positive multiple of KV, max_rows positive");
-    int nt, across;
-    a4_shape((int64_t)max_rows * (H / KV), nt, across);
-    *bytes = (size_t)a4_blocks(nt) * (A4_WARPS / across) * (sizeof(A4Item) + (size_t)2 * 4 * nt * across * (hd + 4) * sizeof(float));
+    const int nt = a4_tiles((int64_t)max_rows * (H / KV));
+    *bytes = (size_t)a4_blocks(nt) * A4_WARPS * (sizeof(A4Item) + (size_t)2 * 4 * nt * (hd + 4) * sizeof(float));
     return B200_OK;
 }
 
@@ -722,11 +727,9 @@ int b200_attention_paged_kv4(const float* q, int64_t q_stride, const int32_t* ro
     rc = b200_attention_paged_kv4_workspace(H, KV, hd, max_rows, &need);
     if (rc) return rc;
     B200_REQUIRE(workspace_bytes >= need, "%s: the workspace has %zu bytes of %zu", who, workspace_bytes, need);
-    int nt, across;
-    a4_shape((int64_t)max_rows * (H / KV), nt, across);
-    const int blocks = a4_blocks(nt), workers = blocks * (A4_WARPS / across);
+    const int nt = a4_tiles((int64_t)max_rows * (H / KV)), blocks = a4_blocks(nt), workers = blocks * A4_WARPS;
     Kv4AttnArgs a{q, q_stride, row_offsets, static_cast<const uint8_t*>(pages), num_pages, page_table, seq_lens, out, out_stride, batch,
-                  max_pages, page, H, KV, H / KV, FastDiv(page), FastDiv(H / KV), FastDiv(4 * nt * across), Kv4Page(page, KV, hd, kind), scale, window, across, 4 * nt * across,
+                  max_pages, page, H, KV, H / KV, FastDiv(page), FastDiv(H / KV), FastDiv(4 * nt), Kv4Page(page, KV, hd, kind), scale, window, 4 * nt,
                   reinterpret_cast<float*>(static_cast<A4Item*>(workspace) + workers), static_cast<A4Item*>(workspace)};
     if (hd == 64)
         rc = kind == 1 ? (nt == 1 ? launch_a4<64, 1, 1>(a, blocks) : launch_a4<64, 1, 2>(a, blocks))
@@ -735,7 +738,7 @@ int b200_attention_paged_kv4(const float* q, int64_t q_stride, const int32_t* ro
         rc = kind == 1 ? (nt == 1 ? launch_a4<128, 1, 1>(a, blocks) : launch_a4<128, 1, 2>(a, blocks))
                        : (nt == 1 ? launch_a4<128, 0, 1>(a, blocks) : launch_a4<128, 0, 2>(a, blocks));
     if (rc) return rc;
-    const dim3 grid(workers, std::max(1, a.pairs * (hd / 4) / A4_JOIN));
+    const dim3 grid(workers);
     return hd == 64 ? launch_serve("attn_kv4_join_kernel", attn_kv4_join_kernel<64>, grid, dim3(A4_JOIN), 0, 1, true, a)
                     : launch_serve("attn_kv4_join_kernel", attn_kv4_join_kernel<128>, grid, dim3(A4_JOIN), 0, 1, true, a);
 }
