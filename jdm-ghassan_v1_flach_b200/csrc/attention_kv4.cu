@@ -24,7 +24,7 @@
 // every block makes by itself.  What a share cuts off an item's ends goes to the workspace and is joined by a second, small kernel.
 // (Shares of whole blocks, their warps joined in shared memory: 74 us where this takes 64.  Warps of a block on different pairs of the
 // same keys: idle ones where the pairs are no multiple, 149 us on the drafts below.)  Keys come through a ring of each warp's own in
-// shared memory that cp.async fills two tiles ahead.
+// shared memory that cp.async fills one or two tiles ahead.
 #include <algorithm>
 
 #include "serve.cuh"
@@ -34,21 +34,13 @@ namespace b200 {
 constexpr int A4_WARPS = 4;
 constexpr int A4_THREADS = A4_WARPS * 32;
 constexpr int A4_KEYS = 32;                      // keys of a warp's step
-#ifndef A4_ITEM
-#define A4_ITEM 2
-#define A4_LEAST 2
-#endif
-#ifndef A4_S1
-#define A4_S1 2
-#define A4_B1 4
-#define A4_S2 3
-#define A4_B2 3
-#endif
-// Stages of a warp's ring and blocks of an SM, by the warp's tiles of four pairs.
-__host__ __device__ constexpr int a4_stages(int nt) { return nt == 1 ? A4_S1 : A4_S2; }
+constexpr int A4_ITEM = 3;                       // what an item's set-up costs, in units
+constexpr int A4_LEAST = 4;                      // units of a worker at the least
+constexpr int A4_RESIDENT = 3;                   // blocks on an SM: 168 registers a thread
+// Stages of a warp's ring, by its tiles of four pairs: two tiles take long enough to hide a load behind one.
+__host__ __device__ constexpr int a4_stages(int nt) { return nt == 1 ? 3 : 2; }
 // A warp's query fragments where they stay in shared memory: 32 registers that two tiles of pairs have more use for.
 __host__ __device__ constexpr int a4_query_bytes(int hd, int nt) { return nt > 1 ? nt * (hd / 32) * 32 * 16 : 0; }
-__host__ __device__ constexpr int a4_resident(int nt) { return nt == 1 ? A4_B1 : A4_B2; }
 
 struct Kv4AttnArgs {
     const float* q;
@@ -105,6 +97,33 @@ __device__ __forceinline__ float a4_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// Two fp32 numbers in a register pair: one instruction for both.
+typedef unsigned long long a4_two;
+__device__ __forceinline__ a4_two a4_both(float a, float b) {
+    a4_two r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 a4_each(a4_two x) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+    return r;
+}
+__device__ __forceinline__ a4_two a4_fma2(a4_two a, a4_two b, a4_two c) {
+    a4_two r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ a4_two a4_mul2(a4_two a, a4_two b) {
+    a4_two r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ a4_two a4_add2(a4_two a, a4_two b) {
+    a4_two r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 __device__ __forceinline__ uint32_t a4_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 template <int BYTES>
@@ -186,7 +205,7 @@ __device__ __forceinline__ A4Range a4_range(const Kv4AttnArgs& a, const A4Seq& s
 }
 
 template <int HD, int KIND, int NT>
-__global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(const __grid_constant__ Kv4AttnArgs a) {
+__global__ void __launch_bounds__(A4_THREADS, A4_RESIDENT) attn_kv4_kernel(const __grid_constant__ Kv4AttnArgs a) {
     using ST = A4Stage<HD, KIND>;
     constexpr int NB = ST::NB, PAIRS = 4 * NT, STAGES = a4_stages(NT), RING = STAGES * ST::BYTES;
     constexpr uint32_t LOW = 0x000F000Fu, UP = 0x00F000F0u;      // code * 2^-24, code * 2^-20
@@ -394,14 +413,15 @@ __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(c
         all_see = __reduce_min_sync(0xffffffffu, all_see);
         none_before = __reduce_max_sync(0xffffffffu, none_before);
 
-        float o[NT][2 * NB][2], bias[NT][NB], m[NT], l[NT];
+        float o[NT][2 * NB][2], m[NT], l[NT];
+        a4_two bias[NT][NB];                                      // of even and odd keys
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             m[j] = -INFINITY;
             l[j] = 0.0f;
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
-                bias[j][n] = 0.0f;
+                bias[j][n] = 0;
                 o[j][2 * n][0] = o[j][2 * n][1] = o[j][2 * n + 1][0] = o[j][2 * n + 1][1] = 0.0f;
             }
         }
@@ -419,7 +439,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(c
             const uint8_t* st = ring + s * ST::BYTES;
 
             // ---- scores ----
-            float x[NT][4];
+            a4_two x2[NT][2];                                     // of key rows g and g + 8
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 uint32_t w[2][NB];                                // of key rows g and g + 8: nibble i of word t's two halves
@@ -441,7 +461,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(c
                     sc[r].load(st + ST::KS + (16 * h + 8 * r + kk) * ST::SROW);
                 }
 #pragma unroll
-                for (int j = 0; j < NT; ++j) x[j][2 * h] = x[j][2 * h + 1] = 0.0f;
+                for (int j = 0; j < NT; ++j) x2[j][h] = 0;
 #pragma unroll
                 for (int n = 0; n < NB; ++n) {
                     const uint32_t s0 = w[0][n] >> 8, s1 = w[1][n] >> 8;
@@ -455,12 +475,8 @@ __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(c
                         if (KIND == 0) a4_mma_from(c, less[j][n][0], less[j][n][1], w[0][n] & LOW, w[1][n] & LOW, w[0][n] & UP, w[1][n] & UP, f.x, f.y);
                         else a4_mma0(c, w[0][n] & LOW, w[1][n] & LOW, w[0][n] & UP, w[1][n] & UP, f.x, f.y);
                         a4_mma(c, s0 & LOW, s1 & LOW, s0 & UP, s1 & UP, f.z, f.w);
-                        x[j][2 * h] = fmaf(d0, c[0] + c[1], x[j][2 * h]);
-                        x[j][2 * h + 1] = fmaf(d1, c[2] + c[3], x[j][2 * h + 1]);
-                        if (KIND == 1) {
-                            x[j][2 * h] = fmaf(m0, qsum[j][n], x[j][2 * h]);
-                            x[j][2 * h + 1] = fmaf(m1, qsum[j][n], x[j][2 * h + 1]);
-                        }
+                        x2[j][h] = a4_fma2(a4_both(d0, d1), a4_both(c[0] + c[1], c[2] + c[3]), x2[j][h]);
+                        if (KIND == 1) x2[j][h] = a4_fma2(a4_both(m0, m1), a4_both(qsum[j][n], qsum[j][n]), x2[j][h]);
                     }
                 }
             }
@@ -470,15 +486,19 @@ __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(c
             float top[NT], here[NT];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
+                float v = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x[j][i] *= unit[j];
+                for (int h = 0; h < 2; ++h) {
+                    x2[j][h] = a4_mul2(x2[j][h], a4_both(unit[j], unit[j]));
+                    float2 x = a4_each(x2[j][h]);
                     if (cut) {
-                        const int key = k + 8 * i + kk;
-                        if (key >= lim[j] || key < from[j]) x[j][i] = -INFINITY;
+                        const int key = k + 16 * h + kk;
+                        if (key >= lim[j] || key < from[j]) x.x = -INFINITY;
+                        if (key + 8 >= lim[j] || key + 8 < from[j]) x.y = -INFINITY;
+                        x2[j][h] = a4_both(x.x, x.y);
                     }
+                    v = fmaxf(v, fmaxf(x.x, x.y));
                 }
-                float v = fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3]));
                 v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
                 v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
                 here[j] = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
@@ -493,7 +513,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(c
                     l[j] *= f;
 #pragma unroll
                     for (int n = 0; n < NB; ++n) {
-                        bias[j][n] *= f;
+                        if (KIND == 1) bias[j][n] = a4_mul2(bias[j][n], a4_both(f, f));
                         o[j][2 * n][0] *= f; o[j][2 * n][1] *= f;
                         o[j][2 * n + 1][0] *= f; o[j][2 * n + 1][1] *= f;
                     }
@@ -510,7 +530,8 @@ __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(c
             }
             if (KIND == 0) top_d = max(top_d & 0xFFFFu, top_d >> 16);
             const float largest = half_bits_to_float((uint16_t)(__reduce_max_sync(0xffffffffu, top_d & 0x7FFFu)));
-            float pg[NT][4], shrink[NT];
+            a4_two pg[NT][2], less_pg[NT][2];                     // weights times grow, and their negatives
+            float shrink[NT];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 const float base = m[j] == -INFINITY ? 0.0f : m[j];
@@ -519,10 +540,14 @@ __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(c
                 const float grow = __uint_as_float((264u - e) << 23);             // 2^(137 - e): p d grow < 2^11
                 shrink[j] = __uint_as_float((14u + e) << 23);                     // 2^24 / grow
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[j][i] = a4_exp2(x[j][i] - base);
-                l[j] += (x[j][0] + x[j][1]) + (x[j][2] + x[j][3]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) pg[j][i] = x[j][i] * grow;
+                for (int h = 0; h < 2; ++h) {
+                    const float2 x = a4_each(a4_add2(x2[j][h], a4_both(-base, -base)));
+                    const float p0 = a4_exp2(x.x), p1 = a4_exp2(x.y);
+                    l[j] += p0 + p1;
+                    x2[j][h] = a4_both(p0, p1);
+                    pg[j][h] = a4_mul2(x2[j][h], a4_both(grow, grow));
+                    less_pg[j][h] = a4_mul2(x2[j][h], a4_both(-grow, -grow));
+                }
             }
             uint32_t vx[8], vy[8];                                // of keys t, t + 4, .. t + 28: the words of dims 4 g .. 4 g + 3
 #pragma unroll
@@ -541,14 +566,19 @@ __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(c
             for (int n = 0; n < NB; ++n) {
                 uint32_t pb[NT][4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float d, mn;
-                    sv[i].get(n, d, mn);
+                for (int h = 0; h < 2; ++h) {
+                    float d0, m0, d1, m1;
+                    sv[2 * h].get(n, d0, m0);
+                    sv[2 * h + 1].get(n, d1, m1);
+                    const a4_two d = a4_both(d0, d1), m8 = KIND == 1 ? a4_fma2(a4_both(8.0f, 8.0f), d, a4_both(m0, m1)) : 0;
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
-                        const float whole = fmaf(pg[j][i], d, ROUND) - ROUND;     // to the nearest whole number
-                        pb[j][i] = a4_turn(a4_pack(whole, fmaf(pg[j][i], d, -whole)));
-                        if (KIND == 1) bias[j][n] = fmaf(x[j][i], fmaf(8.0f, d, mn), bias[j][n]);
+                        // minus the nearest whole number, and what is left: the first column comes out negative
+                        const a4_two less_whole = a4_add2(a4_fma2(less_pg[j][h], d, a4_both(ROUND, ROUND)), a4_both(-ROUND, -ROUND));
+                        const float2 hi = a4_each(less_whole), lo = a4_each(a4_fma2(pg[j][h], d, less_whole));
+                        pb[j][2 * h] = a4_turn(a4_pack(hi.x, lo.x));
+                        pb[j][2 * h + 1] = a4_turn(a4_pack(hi.y, lo.y));
+                        if (KIND == 1) bias[j][n] = a4_fma2(x2[j][h], m8, bias[j][n]);
                     }
                 }
                 uint32_t w[4];
@@ -568,8 +598,8 @@ __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(c
                         float c[4] = {eights[j][0], eights[j][1], eights[j][2], eights[j][3]};
                         a4_mma(c, w[0] & LOW, w[0] & UP, w[1] & LOW, w[1] & UP, pb[j][0], pb[j][1]);
                         a4_mma(c, w[2] & LOW, w[2] & UP, w[3] & LOW, w[3] & UP, pb[j][2], pb[j][3]);
-                        o[j][2 * n + v][0] = fmaf(c[0] + c[1], shrink[j], o[j][2 * n + v][0]);
-                        o[j][2 * n + v][1] = fmaf(c[2] + c[3], shrink[j], o[j][2 * n + v][1]);
+                        o[j][2 * n + v][0] = fmaf(c[1] - c[0], shrink[j], o[j][2 * n + v][0]);
+                        o[j][2 * n + v][1] = fmaf(c[3] - c[2], shrink[j], o[j][2 * n + v][1]);
                     }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) w[i] >>= 8;
@@ -580,12 +610,18 @@ __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(c
         const bool whole = i0 == 0 && i1 == seq.units;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
+            float rest_of[NB];
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                const float2 y = a4_each(bias[j][n]);
+                rest_of[n] = y.x + y.y;
+            }
 #pragma unroll
             for (int sh = 4; sh < 32; sh <<= 1) {
                 l[j] += __shfl_xor_sync(0xffffffffu, l[j], sh);
 #pragma unroll
                 for (int n = 0; n < NB; ++n)
-                    if (KIND == 1) bias[j][n] += __shfl_xor_sync(0xffffffffu, bias[j][n], sh);
+                    if (KIND == 1) rest_of[n] += __shfl_xor_sync(0xffffffffu, rest_of[n], sh);
             }
             const int p = pair0 + 4 * j + t;
             if (p >= npairs) continue;
@@ -596,8 +632,8 @@ __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(c
 #pragma unroll
             for (int n = 0; n < NB; ++n)
                 *reinterpret_cast<float4*>(dst + 32 * n + 4 * g) =
-                    make_float4((o[j][2 * n][0] + bias[j][n]) * mul, fmaf(o[j][2 * n][1], 0.0625f, bias[j][n]) * mul,
-                                (o[j][2 * n + 1][0] + bias[j][n]) * mul, fmaf(o[j][2 * n + 1][1], 0.0625f, bias[j][n]) * mul);
+                    make_float4((o[j][2 * n][0] + rest_of[n]) * mul, fmaf(o[j][2 * n][1], 0.0625f, rest_of[n]) * mul,
+                                (o[j][2 * n + 1][0] + rest_of[n]) * mul, fmaf(o[j][2 * n + 1][1], 0.0625f, rest_of[n]) * mul);
             if (!whole && g == 0) {
                 piece[HD] = m[j];
                 piece[HD + 1] = l[j];
@@ -683,7 +719,7 @@ __global__ void __launch_bounds__(A4_JOIN) attn_kv4_join_kernel(const __grid_con
 
 // Tiles of four pairs that a warp takes at once, from the most pairs that a sequence has for a KV head.
 static int a4_tiles(int64_t most) { return most <= 4 ? 1 : 2; }
-static int a4_blocks(int nt) { return a4_resident(nt) * num_sms(); }
+static int a4_blocks() { return A4_RESIDENT * num_sms(); }
 
 template <int HD, int KIND, int NT>
 static int launch_a4(const Kv4AttnArgs& a, int blocks) {
@@ -705,7 +741,7 @@ int b200_attention_paged_kv4_workspace(int H, int KV, int hd, int max_rows, size
     B200_REQUIRE(bytes, "attention_paged_kv4_workspace: null pointer");
     B200_REQUIRE(H >= 1 && H % KV == 0 && max_rows >= 1, "attention_paged_kv4_workspace: H must be a positive multiple of KV, max_rows positive");
     const int nt = a4_tiles((int64_t)max_rows * (H / KV));
-    *bytes = (size_t)a4_blocks(nt) * A4_WARPS * (sizeof(A4Item) + (size_t)2 * 4 * nt * (hd + 4) * sizeof(float));
+    *bytes = (size_t)a4_blocks() * A4_WARPS * (sizeof(A4Item) + (size_t)2 * 4 * nt * (hd + 4) * sizeof(float));
     return B200_OK;
 }
 
@@ -727,7 +763,7 @@ int b200_attention_paged_kv4(const float* q, int64_t q_stride, const int32_t* ro
     rc = b200_attention_paged_kv4_workspace(H, KV, hd, max_rows, &need);
     if (rc) return rc;
     B200_REQUIRE(workspace_bytes >= need, "%s: the workspace has %zu bytes of %zu", who, workspace_bytes, need);
-    const int nt = a4_tiles((int64_t)max_rows * (H / KV)), blocks = a4_blocks(nt), workers = blocks * A4_WARPS;
+    const int nt = a4_tiles((int64_t)max_rows * (H / KV)), blocks = a4_blocks(), workers = blocks * A4_WARPS;
     Kv4AttnArgs a{q, q_stride, row_offsets, static_cast<const uint8_t*>(pages), num_pages, page_table, seq_lens, out, out_stride, batch,
                   max_pages, page, H, KV, H / KV, FastDiv(page), FastDiv(H / KV), FastDiv(4 * nt), Kv4Page(page, KV, hd, kind), scale, window, 4 * nt,
                   reinterpret_cast<float*>(static_cast<A4Item*>(workspace) + workers), static_cast<A4Item*>(workspace)};
