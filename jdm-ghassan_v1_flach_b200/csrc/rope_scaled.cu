@@ -53,57 +53,76 @@ __device__ __forceinline__ void rs_store(float* p, const RsVec<W>& r) {
 }
 
 // HALVES: pairs (i, i + rot/2), a step is W pairs; else pairs (2i, 2i+1), a step is W elements (W even).
-// Behind the turned part a step copies W elements.  grid (tokens, shares of the heads).
+// Behind the turned part a step copies W elements.  grid (tokens, shares of the heads).  A thread's first steps are loaded before the
+// angles are made, which take as long as the loads do.
 template <bool HALVES, int W>
-__global__ void __launch_bounds__(RS_THREADS) rope_scaled_kernel(RopeArgs a) {
+__global__ void __launch_bounds__(RS_THREADS) rope_scaled_kernel(const __grid_constant__ RopeArgs a) {
+    constexpr int AT_ONCE = 4;
     __shared__ float2 s_cs[RS_MAX_PAIRS];
     const int64_t t = blockIdx.x;
-    const int pos = a.pos[t];
-    if (pos < 0) return;
     const int half = a.rot / 2;
-    for (int i = threadIdx.x; i < half; i += RS_THREADS) {
-        const double turns = (double)pos * (a.freq[i] * 0.15915494309189533577);
-        const double rest = turns - rint(turns);
-        const float r = (float)rest;
-        float s, c;
-        sincospif(2.0f * r, &s, &c);
-        const float d = 6.2831853071795865f * (float)(rest - (double)r);
-        s_cs[i] = make_float2(a.factor * fmaf(-s, d, c), a.factor * fmaf(c, d, s));
-    }
-    __syncthreads();
-    const int turned = HALVES ? half / W : a.rot / W;       // steps that turn, the others copy
-    const int all = (a.heads + a.kv) * a.items;
-    for (int n = blockIdx.y * RS_THREADS + threadIdx.x; n < all; n += gridDim.y * RS_THREADS) {
-        const int h = (int)a.by_items.div(n), j = n - h * a.items;
-        const bool is_q = h < a.heads;
-        const float* src = is_q ? a.q + t * a.qs + (int64_t)h * a.hd : a.k + t * a.ks + (int64_t)(h - a.heads) * a.hd;
-        float* dst = is_q ? a.q_out + t * a.qos + (int64_t)h * a.hd : a.k_out + t * a.kos + (int64_t)(h - a.heads) * a.hd;
-        if (j >= turned) {
-            const int e = a.rot + (j - turned) * W;
-            if (src != dst) rs_store<W>(dst + e, rs_load<W>(src + e));
-        } else if (HALVES) {
-            const int e = j * W;
-            RsVec<W> x = rs_load<W>(src + e), y = rs_load<W>(src + e + half);
+    const int turned = HALVES ? half / W : a.rot / W;       // steps of a head that turn, the others copy
+    const int all = (a.heads + a.kv) * a.items, stride = gridDim.y * RS_THREADS;
+    const float *q = a.q + t * a.qs, *k = a.k + t * a.ks;
+    float *q_out = a.q_out + t * a.qos, *k_out = a.k_out + t * a.kos;
+    const int pos = a.pos[t];
+    bool first = true;
+    for (int n0 = blockIdx.y * RS_THREADS + threadIdx.x; first || n0 < all; n0 += AT_ONCE * stride) {
+        RsVec<W> x[AT_ONCE], y[AT_ONCE];
+        float* to[AT_ONCE];
+        int at[AT_ONCE];                                    // of the pairs' first one; -1: copied, -2: nothing
 #pragma unroll
-            for (int i = 0; i < W; ++i) {
-                const float2 cs = s_cs[e + i];
-                const float u = x.v[i], v = y.v[i];
-                x.v[i] = u * cs.x - v * cs.y;
-                y.v[i] = u * cs.y + v * cs.x;
+        for (int s = 0; s < AT_ONCE; ++s) {
+            const int n = n0 + s * stride;
+            at[s] = -2;
+            if (n >= all) continue;
+            const int h = (int)a.by_items.div(n), j = n - h * a.items;
+            const bool is_q = h < a.heads;
+            const float* src = (is_q ? q : k) + (int64_t)(is_q ? h : h - a.heads) * a.hd;
+            const int e = j < turned ? j * W : a.rot + (j - turned) * W;
+            to[s] = (is_q ? q_out : k_out) + (int64_t)(is_q ? h : h - a.heads) * a.hd + e;
+            x[s] = rs_load<W>(src + e);
+            if (HALVES && j < turned) y[s] = rs_load<W>(src + e + half);
+            at[s] = j >= turned ? (src + e == to[s] ? -2 : -1) : HALVES ? e : e / 2;
+        }
+        if (first) {
+            first = false;
+            if (pos < 0) return;
+            for (int i = threadIdx.x; i < half; i += RS_THREADS) {
+                const double turns = (double)pos * (a.freq[i] * 0.15915494309189533577);
+                const double rest = turns - rint(turns);
+                const float r = (float)rest;
+                float s, c;
+                sincospif(2.0f * r, &s, &c);
+                const float d = 6.2831853071795865f * (float)(rest - (double)r);
+                s_cs[i] = make_float2(a.factor * fmaf(-s, d, c), a.factor * fmaf(c, d, s));
             }
-            rs_store<W>(dst + e, x);
-            rs_store<W>(dst + e + half, y);
-        } else {
-            const int e = j * W;
-            RsVec<W> x = rs_load<W>(src + e);
+            __syncthreads();
+        }
 #pragma unroll
-            for (int i = 0; i + 1 < W; i += 2) {
-                const float2 cs = s_cs[(e + i) / 2];
-                const float u = x.v[i], v = x.v[i + 1];
-                x.v[i] = u * cs.x - v * cs.y;
-                x.v[i + 1] = u * cs.y + v * cs.x;
+        for (int s = 0; s < AT_ONCE; ++s) {
+            if (at[s] == -2) continue;
+            if (at[s] >= 0) {
+                if (HALVES) {
+#pragma unroll
+                    for (int i = 0; i < W; ++i) {
+                        const float2 cs = s_cs[at[s] + i];
+                        const float u = x[s].v[i], v = y[s].v[i];
+                        x[s].v[i] = u * cs.x - v * cs.y;
+                        y[s].v[i] = u * cs.y + v * cs.x;
+                    }
+                    rs_store<W>(to[s] + half, y[s]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i + 1 < W; i += 2) {
+                        const float2 cs = s_cs[at[s] + i / 2];
+                        const float u = x[s].v[i], v = x[s].v[i + 1];
+                        x[s].v[i] = u * cs.x - v * cs.y;
+                        x[s].v[i + 1] = u * cs.y + v * cs.x;
+                    }
+                }
             }
-            rs_store<W>(dst + e, x);
+            rs_store<W>(to[s], x[s]);
         }
     }
 }
