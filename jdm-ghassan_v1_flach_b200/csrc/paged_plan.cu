@@ -5,10 +5,11 @@
 // tail and the offsets are the sums cut off at the last admitted one.  Row r then belongs to the last request whose offset is
 // at most r, found by bisection in shared memory; the same for the pages.
 //
-// What bounds it: latency (a few kilobytes in, 8 bytes per row out).  So it is one launch: a cluster of eight blocks, every one
-// of which reads the requests and sums them by itself, waits until all have read (the outputs may be the inputs), and writes
-// its share.  A step of a few rows takes one block.
-#include <cooperative_groups.h>
+// What bounds it: latency (a few kilobytes in, 8 bytes per row out).  So every block reads the requests and sums them by itself,
+// and writes its share of the rows and pages; the first also what belongs to the requests.  Where those outputs are the inputs and one
+// block is not enough, a second launch of one block writes them when nobody reads any more.
+// (A cluster of eight blocks that waits before it writes: 24.6 us on 700 requests with 88 000 rows.)
+#include <algorithm>
 
 #include "serve.cuh"
 
@@ -31,6 +32,7 @@ struct PlanArgs {
     int32_t *seq_lens, *held_out, *offsets, *positions, *slots;
     int max_rows;
     int32_t* counts;
+    bool expand, report;                         // rows and pages; what belongs to the requests
 };
 
 // Last index in [0, n) whose entry is at most x (s[0] = 0 <= x, s ascending).
@@ -43,8 +45,7 @@ __device__ __forceinline__ int pp_find(const int* s, int n, int x) {
     return lo;
 }
 
-__global__ void __launch_bounds__(PP_THREADS) paged_plan_kernel(PlanArgs a) {
-    namespace cg = cooperative_groups;
+__global__ void __launch_bounds__(PP_THREADS) paged_plan_kernel(const __grid_constant__ PlanArgs a) {
     __shared__ int s_row[PP_BATCH + 1], s_take[PP_BATCH + 1], s_back[PP_BATCH], s_ctx[PP_BATCH], s_held[PP_BATCH];
     __shared__ long long s_part[PP_THREADS / 32][3];
     __shared__ int s_most[2], s_refused;
@@ -139,10 +140,9 @@ __global__ void __launch_bounds__(PP_THREADS) paged_plan_kernel(PlanArgs a) {
         s_row[a.batch] = all_rows;
         s_take[a.batch] = all_take;
     }
-    cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();                              // every block has read what the outputs may overwrite
-    const int rank = (int)cluster.block_rank(), nthreads = (int)cluster.num_blocks() * PP_THREADS, id = rank * PP_THREADS + tid;
-    if (rank == 0) {
+    __syncthreads();                             // everything is read that a single block's outputs may overwrite
+    const int nthreads = gridDim.x * PP_THREADS, id = blockIdx.x * PP_THREADS + tid;
+    if (a.report && blockIdx.x == 0) {
 #pragma unroll
         for (int i = 0; i < PP_EACH; ++i) {
             const int b = tid * PP_EACH + i;
@@ -161,6 +161,7 @@ __global__ void __launch_bounds__(PP_THREADS) paged_plan_kernel(PlanArgs a) {
             a.counts[3] = s_refused;
         }
     }
+    if (!a.expand) return;
     const uint32_t ring_head = sound ? (uint32_t)(head % a.ring_size) : 0, ring_tail = sound ? (uint32_t)(tail % a.ring_size) : 0;
     auto ring_index = [&](uint32_t from, uint32_t j) {      // both below the ring's size
         const uint32_t i = from + j;
@@ -207,7 +208,12 @@ extern "C" int b200_paged_plan(const int32_t* ctx_lens, const int32_t* new_lens,
     B200_REQUIRE(batch == 0 || (ctx_lens && new_lens && held && page_table && seq_lens && held_out), "paged_plan: null pointer");
     B200_REQUIRE(max_rows == 0 || (positions && slots), "paged_plan: null pointer");
     PlanArgs a{ctx_lens, new_lens, held, batch, page_table, max_pages, page, num_pages, FastDiv(page), free_ring, (uint32_t)ring_size,
-               ring_at, ring_at_out, seq_lens, held_out, row_offsets, positions, slots, max_rows, counts};
-    const int blocks = max_rows > 2 * PP_THREADS || batch > 64 ? 8 : 1;
-    return launch_serve("paged_plan_kernel", paged_plan_kernel, dim3(blocks), dim3(PP_THREADS), 0, blocks, false, a);
+               ring_at, ring_at_out, seq_lens, held_out, row_offsets, positions, slots, max_rows, counts, true, true};
+    const int blocks = std::min(num_sms(), std::max(ceil_div(max_rows, 2 * PP_THREADS), ceil_div(batch, 128)));
+    a.report = blocks <= 1 || !(seq_lens == ctx_lens || held_out == held || ring_at_out == ring_at);
+    int rc = launch_serve("paged_plan_kernel", paged_plan_kernel, dim3(std::max(blocks, 1)), dim3(PP_THREADS), 0, 1, false, a);
+    if (rc || a.report) return rc;
+    a.expand = false;
+    a.report = true;
+    return launch_serve("paged_plan_kernel", paged_plan_kernel, dim3(1), dim3(PP_THREADS), 0, 1, false, a);
 }

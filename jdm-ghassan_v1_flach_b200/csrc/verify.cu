@@ -1,20 +1,21 @@
 // Drafted tokens against the target's probabilities, from given uniforms.
 //
-// Two kernels.  The first reads every row of logits once, a chunk of 8192 per block, and leaves its largest value, where that
-// stands, and the sum of exp((l - largest) / T).  The second has a cluster of eight blocks per sequence: each joins the chunks
-// of the sequence's rows by itself (a few hundred words), decides how many drafts are kept, and then sums its eighth of the one row
-// that the next token is drawn from, a segment per warp; the 64 segments' masses are exchanged through the cluster's shared memory,
-// and the warp that holds the draw walks its segment again.  Mass i is e_i - q_i Z with e_i = exp((l_i - max) / T): nothing
-// is divided by Z.
+// Two kernels.  The first reads every row of logits once, a chunk per block, and leaves its largest value, where that stands,
+// and the sum of 2^(l c - R), c = log2(e) / T.  The second has a cluster of eight blocks per sequence: each joins the chunks of the
+// sequence's rows by itself (a few hundred words), decides how many drafts are kept, and then sums its eighth of the one row that the
+// next token is drawn from, a segment per warp; the 64 segments' masses are exchanged through the cluster's shared memory, and
+// the warp that holds the draw walks its segment again.  Mass i is e_i - q_i Z with e_i the weight: nothing is divided by Z.
 //
-// A draw falls on another index than the exact one where u * mass lies within the sums' error of a border, and a flat row has
-// 100 000 borders.  So the argument of exp is kept in two fp32 parts (l - max and its rounding error, 1 / T in two parts), Z
-// in two for e - q Z, and sums run in fp64: what is left is the rounding of single weights, 2^-23 of each with either
-// sign, which moves a border of a flat row by about 1e-10 of the mass.
+// A draw falls on another index than the exact one where u * mass lies within the sums' error of a border, and a row has 100 000 of them:
+// with weights off by 2^-25 of themselves at random, one draw in 10 000 (counted on rows of variance 6).  So a weight is made to 2^-29: the
+// argument as two fp32 numbers, a whole number R taken from it instead of the largest logit (exact, and chunks are
+// joined by powers of two), 2^y = 2^(n/16) 2^f with the sixteen powers kept in two parts and 2^f - 1, at most 1/32, from its series;
+// and sums run in fp64.
 //
-// What bounds it: the logits, once (4 V bytes a row).
+// What bounds it: the logits, once (4 V bytes a row); two dozen instructions a logit make it a near thing.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include <cooperative_groups.h>
 
@@ -26,10 +27,10 @@ namespace cg = cooperative_groups;
 
 constexpr int VD_THREADS = 256;
 constexpr int VD_WARPS = VD_THREADS / 32;
-constexpr int VD_EACH = 32;                       // logits of a thread
-constexpr int VD_CHUNK = VD_THREADS * VD_EACH;
+constexpr int VD_CHUNK = VD_THREADS * 8;          // logits of a chunk at the least, which sizes the workspace
 constexpr int VD_CLUSTER = 8;
 constexpr int VD_MAX_DRAFTS = 255;
+constexpr int VD_ROUND = 64;                      // steps of 128 logits that a block walks at a time
 
 struct VdPart {                                   // of one chunk of one row
     double sum;
@@ -44,24 +45,68 @@ struct VerifyArgs {
     int64_t ds;
     const int32_t *ids, *offsets;
     int batch, rows, V, chunks;
-    float inv_hi, inv_lo;                         // 1 / temperature
+    float c_hi, c_lo;                             // log2(e) / temperature
+    double c;
     const float* uniforms;
     int max_drafts;
     int32_t *accepted, *tokens;
     VdPart* part;
 };
 
-// exp((l - top) / T), 0 for NaN and -inf; l <= top.
-__device__ __forceinline__ float vd_weight(float l, float top, float inv_hi, float inv_lo) {
-    if (l == top) return 1.0f;                    // an infinite top too
-    const float d = __fsub_rn(l, top);
-    // what rounding left of l - top
-    const float b = __fadd_rn(d, top), err = __fsub_rn(__fsub_rn(l, b), __fsub_rn(top, __fsub_rn(b, d)));
-    const float t = __fmul_rn(d, inv_hi);
-    if (!(t > -104.0f)) return 0.0f;              // also NaN, -inf
-    const float low = fmaf(d, inv_hi, -t) + fmaf(d, inv_lo, err * inv_hi);
-    const float e = expf(t);
-    return fmaf(e, low, e);
+// What a row's (or chunk's) weights are taken relative to: weight = 2^((l - s) c - r).  r is whole, and s 0 but for logits so large that l c is
+// no number to work with; there l - s is exact for every l whose weight counts.
+struct VdRef {
+    float s;
+    int r;
+};
+__device__ __forceinline__ VdRef vd_ref(const VerifyArgs& a, float top) {
+    const float y = top * a.c_hi;
+    return fabsf(y) < 30000.0f ? VdRef{0.0f, (int)rintf(y)} : VdRef{top, 0};
+}
+// 2^(from's exponent - to's): sums taken relative to `from` times this are relative to `to`; from <= to.
+__device__ __forceinline__ double vd_rescale(const VerifyArgs& a, float from_top, float to_top) {
+    if (from_top == to_top) return 1.0;
+    if (isinf(to_top) || isinf(from_top)) return 0.0;
+    const VdRef f = vd_ref(a, from_top), t = vd_ref(a, to_top);
+    if (f.s == 0.0f && t.s == 0.0f) {
+        const int d = f.r - t.r;                  // at most 0
+        return d < -1022 ? 0.0 : __hiloint2double((1023 + d) << 20, 0);
+    }
+    return exp2(((double)f.s - (double)t.s) * a.c + (double)(f.r - t.r));
+}
+
+// 2^(k/16), made by every block for itself: the bits of its fp32 value less k << 19, so that adding n << 19 gives 2^(n/16); and
+// what the rounding left, relative to it.
+__device__ __forceinline__ void vd_table(int2* s_pow) {
+    if (threadIdx.x < 16) {
+        const double p = exp2(threadIdx.x / 16.0);
+        s_pow[threadIdx.x] = make_int2(__float_as_int((float)p) - (int)(threadIdx.x << 19), __float_as_int((float)((p - (double)(float)p) / p)));
+    }
+}
+// What the weights of one row or chunk have in common.
+struct VdWeights {
+    const int2* s_pow;
+    float c_hi, c_lo, s, least;                   // below `least` the weight is under 2^-120 of the largest, and 0
+    int shift;                                    // -r, where an exponent stands
+    // The weight of l as hi + lo.  NaN and -inf have none.
+    __device__ __forceinline__ void operator()(float l, float& hi, float& lo) const {
+        constexpr float ROUND = 12582912.0f;      // 1.5 * 2^23
+        const float x = fmaxf(l, least) - s;
+        const float t = __fmul_rn(x, c_hi);
+        const float low = fmaf(x, c_lo, fmaf(x, c_hi, -t));
+        const float z = fmaf(t, 16.0f, ROUND), n = z - ROUND;             // the low bits of z are those of n
+        const float f = fmaf(n, -0.0625f, t) + low;
+        const int i = __float_as_int(z);
+        const int2 p = s_pow[i & 15];
+        const float g = fmaf(f, fmaf(f, fmaf(f, fmaf(f, 9.6181291e-3f, 5.5504109e-2f), 0.24022651f), 0.69314718f), __int_as_float(p.y));   // ln(2)^k / k!
+        hi = l >= least ? __int_as_float(p.x + (i << 19) + shift) : 0.0f;
+        lo = hi * g;
+    }
+};
+__device__ __forceinline__ VdWeights vd_weights(const VerifyArgs& a, const int2* s_pow, float top) {
+    const VdRef ref = vd_ref(a, top);
+    const float least = ref.s + (float)((double)(ref.r - 120) / a.c);
+    return VdWeights{s_pow, a.c_hi, a.c_lo, ref.s, fmaxf(least, -3.402823466e38f), (int)((unsigned)-ref.r << 23)};
 }
 
 struct VdBest {
@@ -79,59 +124,80 @@ __device__ __forceinline__ VdBest vd_warp_best(VdBest a) {
     return a;
 }
 
-// grid (chunks, rows)
-template <bool WIDE, bool GREEDY>
-__global__ void __launch_bounds__(VD_THREADS) verify_stats_kernel(VerifyArgs a) {
-    __shared__ VdBest s_best[VD_WARPS];
-    __shared__ double s_sum[VD_WARPS];
+// grid (chunks, rows); EACH logits of a thread
+template <bool WIDE, bool GREEDY, int EACH>
+__global__ void __launch_bounds__(VD_THREADS) verify_stats_kernel(const __grid_constant__ VerifyArgs a) {
+    __shared__ VdPart s_part[VD_WARPS];
+    __shared__ int2 s_pow[16];
     asm volatile("griddepcontrol.launch_dependents;");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int live = a.offsets[a.batch];
+    bool table = false;
     for (int row = blockIdx.y; row < a.rows; row += gridDim.y) {
-        if (row >= a.offsets[a.batch]) return;
+        if (row >= live) return;
         const float* l = a.logits + row * a.ls;
-        const int c0 = blockIdx.x * VD_CHUNK;
-        float x[VD_EACH];
+        const int c0 = blockIdx.x * (VD_THREADS * EACH);
+        float x[EACH];
         VdBest best{-INFINITY, -1};
 #pragma unroll
-        for (int i = 0; i < VD_EACH; i += 4) {
+        for (int i = 0; i < EACH; i += 4) {
             const int at = c0 + i * VD_THREADS + 4 * threadIdx.x;
             if (WIDE) {
-                const float4 f = at < a.V ? __ldcs(reinterpret_cast<const float4*>(l + at)) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                const float4 f = at < a.V ? *reinterpret_cast<const float4*>(l + at) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
                 x[i] = f.x; x[i + 1] = f.y; x[i + 2] = f.z; x[i + 3] = f.w;
             } else {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) x[i + k] = at + k < a.V ? l[at + k] : -INFINITY;
             }
         }
+        if (!GREEDY && !table) {
+            vd_table(s_pow);
+            table = true;
+        }
+        if (GREEDY) {
 #pragma unroll
-        for (int i = 0; i < VD_EACH; ++i)
-            if (x[i] > best.v) best = VdBest{x[i], c0 + (i & ~3) * VD_THREADS + 4 * (int)threadIdx.x + (i & 3)};
-        best = vd_warp_best(best);
-        if (lane == 0) s_best[warp] = best;
-        __syncthreads();
+            for (int i = 0; i < EACH; ++i)
+                if (x[i] > best.v) best = VdBest{x[i], c0 + (i & ~3) * VD_THREADS + 4 * (int)threadIdx.x + (i & 3)};
+            best = vd_warp_best(best);
+        } else {                                   // where it stands is not asked
 #pragma unroll
-        for (int w = 0; w < VD_WARPS; ++w) best = vd_better(best, s_best[w]);
+            for (int i = 0; i < EACH; ++i) best.v = fmaxf(best.v, x[i]);
+            best.v = warp_max(best.v);
+            best.i = best.v > -INFINITY ? 0 : -1;
+        }
+        __syncthreads();                           // the table is there; the row before is done with s_part
         double sum = 0.0;
         if (!GREEDY && best.i >= 0) {
+            if (best.v == INFINITY) {              // infinite logits share the mass
 #pragma unroll
-            for (int i = 0; i < VD_EACH; i += 4) {
-                float s = 0.0f;
+                for (int i = 0; i < EACH; ++i) sum += x[i] == INFINITY ? 1.0 : 0.0;
+            } else {
+                const VdWeights weigh = vd_weights(a, s_pow, best.v);
+                float rest = 0.0f;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) s += vd_weight(x[i + k], best.v, a.inv_hi, a.inv_lo);
-                sum += (double)s;
+                for (int i = 0; i < EACH; ++i) {
+                    float hi, lo;
+                    weigh(x[i], hi, lo);
+                    sum += (double)hi;
+                    rest += lo;
+                }
+                sum += (double)rest;
             }
             sum = warp_sum_d(sum);
-            if (lane == 0) s_sum[warp] = sum;
-            __syncthreads();
-            sum = 0.0;
-            for (int w = 0; w < VD_WARPS; ++w) sum += s_sum[w];
         }
-        if (threadIdx.x == 0) a.part[(int64_t)row * a.chunks + blockIdx.x] = VdPart{sum, best.v, best.i};
+        if (lane == 0) s_part[warp] = VdPart{sum, best.v, best.i};
         __syncthreads();
+        if (warp == 0) {
+            const VdPart p = s_part[lane % VD_WARPS];
+            best = vd_warp_best(VdBest{p.top, p.at});
+            sum = !GREEDY && lane < VD_WARPS && p.at >= 0 ? p.sum * vd_rescale(a, p.top, best.v) : 0.0;
+            sum = warp_sum_d(sum);
+            if (lane == 0) a.part[(int64_t)row * a.chunks + blockIdx.x] = VdPart{sum, best.v, best.i};
+        }
     }
 }
 
-// One warp: a row's arg-max and, for the largest value, Z.
+// One warp: a row's arg-max and Z relative to it.
 template <bool GREEDY>
 __device__ __forceinline__ void vd_join(const VerifyArgs& a, int row, int lane, VdBest& best, double& z) {
     const VdPart* p = a.part + (int64_t)row * a.chunks;
@@ -140,25 +206,25 @@ __device__ __forceinline__ void vd_join(const VerifyArgs& a, int row, int lane, 
     best = vd_warp_best(best);
     z = 0.0;
     if (!GREEDY) {
-        for (int c = lane; c < a.chunks; c += 32) {
-            const float top = __ldcg(&p[c].top);
-            if (__ldcg(&p[c].at) < 0) continue;
-            const double t = top == best.v ? 0.0 : ((double)top - (double)best.v) * ((double)a.inv_hi + (double)a.inv_lo);
-            z += __ldcg(&p[c].sum) * exp(t);
-        }
+        for (int c = lane; c < a.chunks; c += 32)
+            if (__ldcg(&p[c].at) >= 0) z += __ldcg(&p[c].sum) * vd_rescale(a, __ldcg(&p[c].top), best.v);
         z = warp_sum_d(z);
     }
 }
 
 // grid (8 per sequence); a cluster has a sequence
 template <bool WIDE, bool GREEDY>
-__global__ void __launch_bounds__(VD_THREADS) verify_pick_kernel(VerifyArgs a) {
+__global__ void __launch_bounds__(VD_THREADS) verify_pick_kernel(const __grid_constant__ VerifyArgs a) {
     __shared__ bool s_keep[VD_MAX_DRAFTS + 1];
     __shared__ float s_top[VD_MAX_DRAFTS + 1];
     __shared__ int s_at[VD_MAX_DRAFTS + 1];
     __shared__ double s_z[VD_MAX_DRAFTS + 1], s_mass[2][VD_WARPS];
+    __shared__ int2 s_pow[16];
+    __shared__ double s_step[VD_ROUND];
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = (int)cluster.block_rank(), b = blockIdx.x / VD_CLUSTER, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    vd_table(s_pow);
+    __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int first = max(a.offsets[b], 0), count = min(a.offsets[b + 1], a.rows) - first, drafts = min(count - 1, a.max_drafts);
     int32_t* tokens = a.tokens + (int64_t)b * (a.max_drafts + 1);
@@ -172,19 +238,19 @@ __global__ void __launch_bounds__(VD_THREADS) verify_pick_kernel(VerifyArgs a) {
     for (int j = warp; j <= drafts; j += VD_WARPS) {
         VdBest best;
         double z;
+        const int x = j < drafts ? a.ids[first + j + 1] : -1;
+        const bool there = (uint32_t)x < (uint32_t)a.V;
+        const float l = !GREEDY && there ? a.logits[(first + j) * a.ls + x] : 0.0f, q = !GREEDY && there && a.draft ? a.draft[(first + j) * a.ds + x] : 1.0f;
+        const float u = !GREEDY && there ? a.uniforms[first + j] : 0.0f;
         vd_join<GREEDY>(a, first + j, lane, best, z);
         if (lane == 0) {
             bool keep = false;
-            if (j < drafts) {
-                const int x = a.ids[first + j + 1];
-                if (GREEDY) {
-                    keep = best.i >= 0 && best.i == x;
-                } else if ((uint32_t)x < (uint32_t)a.V && best.i >= 0) {
-                    const float l = a.logits[(first + j) * a.ls + x];
-                    const double e = (double)vd_weight(l, best.v, a.inv_hi, a.inv_lo), u = (double)a.uniforms[first + j];
-                    const double q = a.draft ? (double)a.draft[(first + j) * a.ds + x] : 1.0;
-                    keep = u * q * z < e;
-                }
+            if (GREEDY) {
+                keep = there && best.i == x;
+            } else if (there && best.i >= 0) {
+                float hi = l == INFINITY ? 1.0f : 0.0f, lo = 0.0f;
+                if (best.v < INFINITY) vd_weights(a, s_pow, best.v)(l, hi, lo);
+                keep = (double)u * (double)q * z < (double)hi + (double)lo;
             }
             s_keep[j] = keep;
             s_top[j] = best.v;
@@ -195,94 +261,155 @@ __global__ void __launch_bounds__(VD_THREADS) verify_pick_kernel(VerifyArgs a) {
     __syncthreads();
     int n = 0;
     while (n < drafts && s_keep[n]) ++n;
-    int next = s_at[n];
+    const int next = s_at[n];
     if (!GREEDY && next >= 0) {
         const int row = first + n;
         const bool refused = n < drafts;
         const float* l = a.logits + row * a.ls;
         const float* q = refused && a.draft ? a.draft + row * a.ds : nullptr;
         const int without = refused && !a.draft ? a.ids[row + 1] : -1;
-        const float top = s_top[n], zh = (float)s_z[n], zl = (float)(s_z[n] - (double)zh);
+        const float top = s_top[n];
+        const double z = s_z[n];
+        const VdWeights weigh = vd_weights(a, s_pow, top);
         // segment of a warp: whole steps of 128 logits
         const int steps = ((a.V + 127) / 128 + VD_CLUSTER * VD_WARPS - 1) / (VD_CLUSTER * VD_WARPS), seg = steps * 128;
-        auto masses = [&](int at, bool from_p, float (&r)[4]) {
-            float x[4], y[4] = {0.f, 0.f, 0.f, 0.f};
+        struct Four {
+            float4 l, q;
+        };
+        auto load = [&](int at) {
+            Four f{make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY), make_float4(0.f, 0.f, 0.f, 0.f)};
             if (WIDE) {
-                const float4 f = at < a.V ? __ldg(reinterpret_cast<const float4*>(l + at)) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-                x[0] = f.x; x[1] = f.y; x[2] = f.z; x[3] = f.w;
-                if (q && at < a.V) {
-                    const float4 g = __ldg(reinterpret_cast<const float4*>(q + at));
-                    y[0] = g.x; y[1] = g.y; y[2] = g.z; y[3] = g.w;
+                if (at < a.V) {
+                    f.l = __ldg(reinterpret_cast<const float4*>(l + at));
+                    if (q) f.q = __ldg(reinterpret_cast<const float4*>(q + at));
                 }
             } else {
+                float *x = &f.l.x, *y = &f.q.x;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    x[k] = at + k < a.V ? l[at + k] : -INFINITY;
-                    if (q && at + k < a.V) y[k] = q[at + k];
-                }
+                for (int k = 0; k < 4; ++k)
+                    if (at + k < a.V) {
+                        x[k] = l[at + k];
+                        if (q) y[k] = q[at + k];
+                    }
             }
+            return f;
+        };
+        auto masses = [&](int at, const Four& f, bool from_p, double (&r)[4]) {
+            const float x[4] = {f.l.x, f.l.y, f.l.z, f.l.w}, y[4] = {f.q.x, f.q.y, f.q.z, f.q.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const float e = vd_weight(x[k], top, a.inv_hi, a.inv_lo);
-                r[k] = from_p ? e : at + k == without ? 0.0f : fmaxf(fmaf(-y[k], zl, fmaf(-y[k], zh, e)), 0.0f);
+                float hi = x[k] == INFINITY ? 1.0f : 0.0f, lo = 0.0f;
+                if (top < INFINITY) weigh(x[k], hi, lo);
+                r[k] = (double)hi + (double)lo;
+                if (!from_p && q) {
+                    r[k] = fma(-(double)y[k], z, r[k]);
+                    if (!(r[k] > 0.0)) r[k] = 0.0;
+                }
+                if (!from_p && at + k == without) r[k] = 0.0;
             }
         };
         const int own = (rank * VD_WARPS + warp) * seg;
         bool from_p = !refused;
-        double before = 0.0, total = 0.0;
+        double lane_from = 0.0, lane_mid = 0.0, lane_to = 0.0, total = 0.0;
         for (int pass = 0; pass < 2; ++pass) {                // the second only where max(p - q, 0) has no mass
             double sum = 0.0;
-            for (int s = 0; s < steps; ++s) {
-                float r[4];
-                masses(own + s * 128 + 4 * lane, from_p, r);
-                sum += ((double)r[0] + (double)r[1]) + ((double)r[2] + (double)r[3]);
+            constexpr int AHEAD = 4;
+            for (int s0 = 0; s0 < steps; s0 += AHEAD) {
+                Four f[AHEAD];
+#pragma unroll
+                for (int s = 0; s < AHEAD; ++s) f[s] = load(s0 + s < steps ? own + (s0 + s) * 128 + 4 * lane : a.V);
+#pragma unroll
+                for (int s = 0; s < AHEAD; ++s) {
+                    if (s0 + s >= steps) break;
+                    double r[4];
+                    masses(own + (s0 + s) * 128 + 4 * lane, f[s], from_p, r);
+                    sum += (r[0] + r[1]) + (r[2] + r[3]);
+                }
             }
             sum = warp_sum_d(sum);
             if (lane == 0) s_mass[pass][warp] = sum;
             cluster.sync();
-            total = 0.0;
-            for (int i = 0; i < VD_CLUSTER * VD_WARPS; ++i) {
-                if (i == rank * VD_WARPS + warp) before = total;
-                total += cluster.map_shared_rank(&s_mass[pass][0], i / VD_WARPS)[i % VD_WARPS];
+            // where the segments begin and end on the line of masses, the same numbers in every warp: lane k has segments 2 k and
+            // 2 k + 1, [prev, mid) and [mid, upto), made to ascend whatever the sums' rounding
+            const double* of = cluster.map_shared_rank(&s_mass[pass][0], lane / 4) + 2 * (lane % 4);
+            const double m0 = of[0], m1 = of[1];
+            double upto = m0 + m1;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const double v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
             }
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const double v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto = fmax(upto, v);
+            }
+            total = __shfl_sync(0xffffffffu, upto, 31);
+            const double up = __shfl_up_sync(0xffffffffu, upto, 1), prev = lane == 0 ? 0.0 : up, mid = fmin(prev + m0, upto);
+            lane_from = prev;
+            lane_mid = mid;
+            lane_to = upto;
             if (total > 0.0 || from_p) break;
             from_p = true;
         }
         const float u = a.uniforms[first + count - 1];
         const double mark = (u > 0.0f ? fmin((double)u, 1.0 - 1.0 / 16777216.0) : 0.0) * total;
-        const double mine = s_mass[from_p && refused ? 1 : 0][warp];
-        if (before <= mark && mark < before + mine) {
-            // this warp's segment holds the draw
-            double run = before;
-            int found = -1, last = -1;
-            for (int s = 0; s < steps && found < 0; ++s) {
-                float r[4];
-                const int at = own + s * 128 + 4 * lane;
-                masses(at, from_p, r);
-                const double sum = ((double)r[0] + (double)r[1]) + ((double)r[2] + (double)r[3]);
+        const unsigned even = __ballot_sync(0xffffffffu, lane_from <= mark && mark < lane_mid), odd = __ballot_sync(0xffffffffu, lane_mid <= mark && mark < lane_to);
+        const int holder = even ? __ffs(even) - 1 : __ffs(odd) - 1;                  // lane whose segments hold the draw: there is one
+        const int which = 2 * holder + (even == 0);
+        if (which / VD_WARPS == rank) {            // this block walks the segment again, its warps a step each
+            double run = __shfl_sync(0xffffffffu, even ? lane_from : lane_mid, holder);
+            const int from = which * seg;
+            int found = -1;                        // the step that holds the draw, or so far the last one that has mass
+            double found_run = 0.0;
+            bool sure = false;
+            for (int s0 = 0; s0 < steps && !sure; s0 += VD_ROUND) {
+                const int here = min(VD_ROUND, steps - s0);
+                for (int s = warp; s < here; s += VD_WARPS) {
+                    const int at = from + (s0 + s) * 128 + 4 * lane;
+                    double r[4];
+                    masses(at, load(at), from_p, r);
+                    const double sum = warp_sum_d((r[0] + r[1]) + (r[2] + r[3]));
+                    if (lane == 0) s_step[s] = sum;
+                }
+                __syncthreads();
+                for (int s = 0; s < here && !sure; ++s) {       // every thread alike
+                    const double m = s_step[s];
+                    if (m > 0.0) {
+                        found = s0 + s;
+                        found_run = run;
+                        sure = run + m > mark;
+                    }
+                    run += m;
+                }
+                __syncthreads();
+            }
+            if (warp == 0) {
+                const int at = from + found * 128 + 4 * lane;
+                double r[4];
+                masses(at, load(at), from_p, r);
+                const double sum = (r[0] + r[1]) + (r[2] + r[3]);
                 double incl = sum;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
-                    const double u = __shfl_up_sync(0xffffffffu, incl, o);
-                    if (lane >= o) incl += u;
+                    const double v = __shfl_up_sync(0xffffffffu, incl, o);
+                    if (lane >= o) incl += v;
                 }
-                double c = run + (incl - sum);
-                int hit = 0x7fffffff, any = -1;
+                double c = found_run + (incl - sum);
+                int hit = 0x7fffffff, last = -1;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    c += (double)r[k];
-                    if (r[k] > 0.0f) {
-                        any = at + k;
+                    c += r[k];
+                    if (r[k] > 0.0) {
+                        last = at + k;
                         if (c > mark) hit = min(hit, at + k);
                     }
                 }
                 hit = __reduce_min_sync(0xffffffffu, hit);
-                any = __reduce_max_sync(0xffffffffu, any);
-                if (hit != 0x7fffffff) found = hit;
-                last = max(last, any);
-                run += __shfl_sync(0xffffffffu, incl, 31);
+                last = __reduce_max_sync(0xffffffffu, last);
+                // sums in another order may end a rounding short of the mark: the last one that has mass
+                if (lane == 0) tokens[n] = hit != 0x7fffffff ? hit : last;
             }
-            if (lane == 0) tokens[n] = found >= 0 ? found : last;     // sums in another order: the segment's last one
         }
         cluster.sync();                            // nobody leaves while its masses are read
     } else if (rank == 0 && threadIdx.x == 0) {
@@ -324,18 +451,25 @@ int b200_verify_drafts(const float* logits, int64_t logits_stride, const float* 
     B200_REQUIRE(temperature == temperature && temperature < INFINITY, "%s: the temperature must be a finite number", who);
     B200_REQUIRE(aligned16(workspace) && workspace_bytes >= need, "%s: the workspace must be 16-byte aligned and have %zu bytes", who, need);
     const bool greedy = temperature <= 0.0f;
-    const double inv = greedy ? 0.0 : 1.0 / (double)temperature;
-    const float hi = (float)inv;
+    const double c = greedy ? 0.0 : 1.4426950408889634 / (double)temperature;
+    const float hi = (float)c;
     B200_REQUIRE(hi < INFINITY, "%s: the temperature is too small", who);
-    VerifyArgs a{logits, logits_stride, draft_probs, draft_stride, ids, row_offsets, batch, rows, V, ceil_div(V, VD_CHUNK),
-                 hi, (float)(inv - (double)hi), uniforms, max_drafts, accepted, tokens, static_cast<VdPart*>(workspace)};
+    VerifyArgs a{logits, logits_stride, draft_probs, draft_stride, ids, row_offsets, batch, rows, V, 0,
+                 hi, (float)(c - (double)hi), c, uniforms, max_drafts, accepted, tokens, static_cast<VdPart*>(workspace)};
     const bool wide = aligned16(logits) && V % 4 == 0 && logits_stride % 4 == 0 &&
                       (!draft_probs || (aligned16(draft_probs) && draft_stride % 4 == 0));
     const dim3 block(VD_THREADS);
     if (rows > 0) {
+        // chunks of 8192 where they fill the device: a quarter of the blocks' fixed costs; else of 2048
+        const bool many = (int64_t)rows * ceil_div(V, 4 * VD_CHUNK) >= 2 * num_sms();
+        a.chunks = ceil_div(V, many ? 4 * VD_CHUNK : VD_CHUNK);
         const dim3 grid(a.chunks, std::min(rows, 65535));
-        auto kern = wide ? (greedy ? verify_stats_kernel<true, true> : verify_stats_kernel<true, false>)
-                         : (greedy ? verify_stats_kernel<false, true> : verify_stats_kernel<false, false>);
+        auto pick = [&](auto each) {
+            constexpr int E = decltype(each)::value;
+            return wide ? (greedy ? verify_stats_kernel<true, true, E> : verify_stats_kernel<true, false, E>)
+                        : (greedy ? verify_stats_kernel<false, true, E> : verify_stats_kernel<false, false, E>);
+        };
+        auto kern = many ? pick(std::integral_constant<int, 32>()) : pick(std::integral_constant<int, 8>());
         rc = launch_serve("verify_stats_kernel", kern, grid, block, 0, 1, false, a);
         if (rc) return rc;
     }

@@ -536,7 +536,7 @@ def test_verify_of_banned_infinite_and_missing_logits(T):
     V = 300
     r = np.random.default_rng(8)
     base = r.standard_normal((1, V)).astype(np.float32)
-    rows = np.repeat(base, 8, 0)
+    rows = np.repeat(base, 9, 0)
     rows[0, :] = -np.inf                               # nothing allowed
     rows[1, 5:] = -np.inf
     rows[2, ::2] = np.nan
@@ -545,17 +545,32 @@ def test_verify_of_banned_infinite_and_missing_logits(T):
     rows[5, 17] = np.inf
     rows[6, :] = -3e38
     rows[7, :200] = -np.inf
-    offsets = np.arange(9)
-    u = np.array([0.3, 0.99, 0.5, 0.7, 0.1, 0.2, 0.6, 0.0])
-    got = run_verify(rows, None, [0] * 8, offsets, T, u, 0)
-    check_verify(rows, None, [0] * 8, offsets, T, u, 0, got)
+    rows[8, :] = -np.finfo(np.float32).max             # the type's lowest, and one beside it that is not
+    rows[8, 123] = 0
+    offsets = np.arange(10)
+    u = np.array([0.3, 0.99, 0.5, 0.7, 0.1, 0.2, 0.6, 0.0, 0.9])
+    got = run_verify(rows, None, [0] * 9, offsets, T, u, 0)
+    check_verify(rows, None, [0] * 9, offsets, T, u, 0, got)
     assert got[1][0, 0] == -1 and got[1][4, 0] == -1
     if T > 0:
         assert got[1][3, 0] == 250 and got[1][5, 0] == 17
     # drafts: one that is banned, ids that are none, a row without logits in the middle
-    ids = [0, 9, -1, V, 17, 17, 3, 3]
-    offs = [0, 2, 4, 8]
-    check_verify(rows, None, ids, offs, T, u, 3, run_verify(rows, None, ids, offs, T, u, 3))
+    ids = [0, 9, -1, V, 17, 17, 3, 3, 123]
+    offs = [0, 2, 4, 9]
+    check_verify(rows, None, ids, offs, T, u, 4, run_verify(rows, None, ids, offs, T, u, 4))
+
+
+@pytest.mark.parametrize("scale,T", [(1e4, 0.01), (3e37, 1e30), (1e-3, 1e-4), (1.0, 1e-20), (1e5, 1.0)])
+def test_verify_of_logits_of_all_sizes(scale, T):
+    """Exponents of thousands and of 1e20, above and below zero: what a weight is taken relative to."""
+    r = np.random.default_rng(11)
+    n, V = 12, 700
+    logits = ((r.standard_normal((n, V)) + np.where(np.arange(n) % 3 == 0, 6, -6)[:, None]) * scale).astype(np.float32)
+    logits[:, 5] = logits.max(1)                       # two that share the mass, and some near them
+    logits[:, 6:9] = (logits[:, 5:6].astype(np.float64) - T * np.array([0.1, 1.0, 3.0])).astype(np.float32)
+    u = (np.arange(n) + 0.37) / n
+    got = run_verify(logits, None, [0] * n, np.arange(n + 1), T, u, 0)
+    check_verify(logits, None, [0] * n, np.arange(n + 1), np.float64(np.float32(T)), u, 0, got)
 
 
 def test_verify_falls_back_where_the_rest_has_no_mass():
