@@ -105,7 +105,7 @@ int b200_attention_paged_kv4(const float* q, int64_t q_stride, const int32_t* ro
 
 /* Drafted tokens against the target's probabilities.  Row row_offsets[b] + j holds the target's logits after the j-th token
  * of sequence b that was fed this step, ids[row_offsets[b] + j]: the drafts are the ids of its second and later rows, checked
- * by the row before.  p = softmax(logits / temperature) (temperature <= 0: greedy); q: the row of draft_probs [rows, V] that the
+ * by the row before.  p = softmax(logits / temperature) (temperature <= 0: greedy, at most 1e30); q: the row of draft_probs [rows, V] that the
  * draft was drawn from (NULL: the drafter had no choice, q(x) = 1).  Draft x is kept iff u * q(x) < p(x), u = uniforms of the
  * checking row, in [0, 1); the first refusal draws from max(p - q, 0) (q = 1 at x alone if draft_probs is NULL), and if there is none
  * the next token is drawn from the last row's p: the first index whose cumulated mass exceeds u * (all of it), u = the

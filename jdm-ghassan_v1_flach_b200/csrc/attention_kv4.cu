@@ -98,33 +98,6 @@ __device__ __forceinline__ float a4_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Two fp32 numbers in a register pair: one instruction for both.
-typedef unsigned long long a4_two;
-__device__ __forceinline__ a4_two a4_both(float a, float b) {
-    a4_two r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 a4_each(a4_two x) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
-    return r;
-}
-__device__ __forceinline__ a4_two a4_fma2(a4_two a, a4_two b, a4_two c) {
-    a4_two r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ a4_two a4_mul2(a4_two a, a4_two b) {
-    a4_two r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ a4_two a4_add2(a4_two a, a4_two b) {
-    a4_two r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 __device__ __forceinline__ uint32_t a4_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 template <int BYTES>
 __device__ __forceinline__ void a4_copy(uint32_t dst, const uint8_t* src) {
@@ -217,9 +190,9 @@ __global__ void __launch_bounds__(A4_THREADS, A4_RESIDENT) attn_kv4_kernel(const
     asm volatile("griddepcontrol.launch_dependents;");
 
     // ---- this worker's share of the units ----
-    const int each = (a.batch + A4_THREADS - 1) / A4_THREADS;
+    const int share = (a.batch + A4_THREADS - 1) / A4_THREADS;
     int64_t mine = 0;
-    for (int i = threadIdx.x * each; i < min(a.batch, (int)(threadIdx.x + 1) * each); ++i) mine += a4_units(a, a4_seq(a, i));
+    for (int i = threadIdx.x * share; i < min(a.batch, (int)(threadIdx.x + 1) * share); ++i) mine += a4_units(a, a4_seq(a, i));
     int64_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -247,7 +220,7 @@ __global__ void __launch_bounds__(A4_THREADS, A4_RESIDENT) attn_kv4_kernel(const
 #pragma unroll
     for (int i = 0; i < A4_WARPS; ++i) b += __popc(__ballot_sync(0xffffffffu, s_from[32 * i + lane] <= u));
     int64_t rest = u - s_from[b];
-    b *= each;
+    b *= share;
     A4Seq seq = a4_seq(a, b);
     while (rest >= a4_units(a, seq)) {
         rest -= a4_units(a, seq);
@@ -414,7 +387,7 @@ __global__ void __launch_bounds__(A4_THREADS, A4_RESIDENT) attn_kv4_kernel(const
         none_before = __reduce_max_sync(0xffffffffu, none_before);
 
         float o[NT][2 * NB][2], m[NT], l[NT];
-        a4_two bias[NT][NB];                                      // of even and odd keys
+        f32x2 bias[NT][NB];                                      // of even and odd keys
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             m[j] = -INFINITY;
@@ -439,7 +412,7 @@ __global__ void __launch_bounds__(A4_THREADS, A4_RESIDENT) attn_kv4_kernel(const
             const uint8_t* st = ring + s * ST::BYTES;
 
             // ---- scores ----
-            a4_two x2[NT][2];                                     // of key rows g and g + 8
+            f32x2 x2[NT][2];                                     // of key rows g and g + 8
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 uint32_t w[2][NB];                                // of key rows g and g + 8: nibble i of word t's two halves
@@ -475,8 +448,8 @@ __global__ void __launch_bounds__(A4_THREADS, A4_RESIDENT) attn_kv4_kernel(const
                         if (KIND == 0) a4_mma_from(c, less[j][n][0], less[j][n][1], w[0][n] & LOW, w[1][n] & LOW, w[0][n] & UP, w[1][n] & UP, f.x, f.y);
                         else a4_mma0(c, w[0][n] & LOW, w[1][n] & LOW, w[0][n] & UP, w[1][n] & UP, f.x, f.y);
                         a4_mma(c, s0 & LOW, s1 & LOW, s0 & UP, s1 & UP, f.z, f.w);
-                        x2[j][h] = a4_fma2(a4_both(d0, d1), a4_both(c[0] + c[1], c[2] + c[3]), x2[j][h]);
-                        if (KIND == 1) x2[j][h] = a4_fma2(a4_both(m0, m1), a4_both(qsum[j][n], qsum[j][n]), x2[j][h]);
+                        x2[j][h] = fma2(two(d0, d1), two(c[0] + c[1], c[2] + c[3]), x2[j][h]);
+                        if (KIND == 1) x2[j][h] = fma2(two(m0, m1), two(qsum[j][n], qsum[j][n]), x2[j][h]);
                     }
                 }
             }
@@ -489,13 +462,13 @@ __global__ void __launch_bounds__(A4_THREADS, A4_RESIDENT) attn_kv4_kernel(const
                 float v = -INFINITY;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    x2[j][h] = a4_mul2(x2[j][h], a4_both(unit[j], unit[j]));
-                    float2 x = a4_each(x2[j][h]);
+                    x2[j][h] = mul2(x2[j][h], two(unit[j], unit[j]));
+                    float2 x = each(x2[j][h]);
                     if (cut) {
                         const int key = k + 16 * h + kk;
                         if (key >= lim[j] || key < from[j]) x.x = -INFINITY;
                         if (key + 8 >= lim[j] || key + 8 < from[j]) x.y = -INFINITY;
-                        x2[j][h] = a4_both(x.x, x.y);
+                        x2[j][h] = two(x.x, x.y);
                     }
                     v = fmaxf(v, fmaxf(x.x, x.y));
                 }
@@ -513,7 +486,7 @@ __global__ void __launch_bounds__(A4_THREADS, A4_RESIDENT) attn_kv4_kernel(const
                     l[j] *= f;
 #pragma unroll
                     for (int n = 0; n < NB; ++n) {
-                        if (KIND == 1) bias[j][n] = a4_mul2(bias[j][n], a4_both(f, f));
+                        if (KIND == 1) bias[j][n] = mul2(bias[j][n], two(f, f));
                         o[j][2 * n][0] *= f; o[j][2 * n][1] *= f;
                         o[j][2 * n + 1][0] *= f; o[j][2 * n + 1][1] *= f;
                     }
@@ -530,7 +503,7 @@ __global__ void __launch_bounds__(A4_THREADS, A4_RESIDENT) attn_kv4_kernel(const
             }
             if (KIND == 0) top_d = max(top_d & 0xFFFFu, top_d >> 16);
             const float largest = half_bits_to_float((uint16_t)(__reduce_max_sync(0xffffffffu, top_d & 0x7FFFu)));
-            a4_two pg[NT][2], less_pg[NT][2];                     // weights times grow, and their negatives
+            f32x2 pg[NT][2], less_pg[NT][2];                     // weights times grow, and their negatives
             float shrink[NT];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
@@ -541,12 +514,12 @@ __global__ void __launch_bounds__(A4_THREADS, A4_RESIDENT) attn_kv4_kernel(const
                 shrink[j] = __uint_as_float((14u + e) << 23);                     // 2^24 / grow
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const float2 x = a4_each(a4_add2(x2[j][h], a4_both(-base, -base)));
+                    const float2 x = each(add2(x2[j][h], two(-base, -base)));
                     const float p0 = a4_exp2(x.x), p1 = a4_exp2(x.y);
                     l[j] += p0 + p1;
-                    x2[j][h] = a4_both(p0, p1);
-                    pg[j][h] = a4_mul2(x2[j][h], a4_both(grow, grow));
-                    less_pg[j][h] = a4_mul2(x2[j][h], a4_both(-grow, -grow));
+                    x2[j][h] = two(p0, p1);
+                    pg[j][h] = mul2(x2[j][h], two(grow, grow));
+                    less_pg[j][h] = mul2(x2[j][h], two(-grow, -grow));
                 }
             }
             uint32_t vx[8], vy[8];                                // of keys t, t + 4, .. t + 28: the words of dims 4 g .. 4 g + 3
@@ -570,15 +543,15 @@ __global__ void __launch_bounds__(A4_THREADS, A4_RESIDENT) attn_kv4_kernel(const
                     float d0, m0, d1, m1;
                     sv[2 * h].get(n, d0, m0);
                     sv[2 * h + 1].get(n, d1, m1);
-                    const a4_two d = a4_both(d0, d1), m8 = KIND == 1 ? a4_fma2(a4_both(8.0f, 8.0f), d, a4_both(m0, m1)) : 0;
+                    const f32x2 d = two(d0, d1), m8 = KIND == 1 ? fma2(two(8.0f, 8.0f), d, two(m0, m1)) : 0;
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
                         // minus the nearest whole number, and what is left: the first column comes out negative
-                        const a4_two less_whole = a4_add2(a4_fma2(less_pg[j][h], d, a4_both(ROUND, ROUND)), a4_both(-ROUND, -ROUND));
-                        const float2 hi = a4_each(less_whole), lo = a4_each(a4_fma2(pg[j][h], d, less_whole));
+                        const f32x2 less_whole = add2(fma2(less_pg[j][h], d, two(ROUND, ROUND)), two(-ROUND, -ROUND));
+                        const float2 hi = each(less_whole), lo = each(fma2(pg[j][h], d, less_whole));
                         pb[j][2 * h] = a4_turn(a4_pack(hi.x, lo.x));
                         pb[j][2 * h + 1] = a4_turn(a4_pack(hi.y, lo.y));
-                        if (KIND == 1) bias[j][n] = a4_fma2(x2[j][h], m8, bias[j][n]);
+                        if (KIND == 1) bias[j][n] = fma2(x2[j][h], m8, bias[j][n]);
                     }
                 }
                 uint32_t w[4];
@@ -613,7 +586,7 @@ __global__ void __launch_bounds__(A4_THREADS, A4_RESIDENT) attn_kv4_kernel(const
             float rest_of[NB];
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
-                const float2 y = a4_each(bias[j][n]);
+                const float2 y = each(bias[j][n]);
                 rest_of[n] = y.x + y.y;
             }
 #pragma unroll

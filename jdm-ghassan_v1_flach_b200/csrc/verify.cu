@@ -4,18 +4,16 @@
 // and the sum of 2^(l c - R), c = log2(e) / T.  The second has a cluster of eight blocks per sequence: each joins the chunks of the
 // sequence's rows by itself (a few hundred words), decides how many drafts are kept, and then sums its eighth of the one row that the
 // next token is drawn from, a segment per warp; the 64 segments' masses are exchanged through the cluster's shared memory, and
-// the warp that holds the draw walks its segment again.  Mass i is e_i - q_i Z with e_i the weight: nothing is divided by Z.
+// the block that holds the draw walks its segment again.  Mass i is e_i - q_i Z with e_i the weight: nothing is divided by Z.
 //
-// A draw falls on another index than the exact one where u * mass lies within the sums' error of a border, and a row has 100 000 of them:
-// with weights off by 2^-25 of themselves at random, one draw in 10 000 (counted on rows of variance 6).  So a weight is made to 2^-29: the
-// argument as two fp32 numbers, a whole number R taken from it instead of the largest logit (exact, and chunks are
-// joined by powers of two), 2^y = 2^(n/16) 2^f with the sixteen powers kept in two parts and 2^f - 1, at most 1/32, from its series;
-// and sums run in fp64.
-//
-// What bounds it: the logits, once (4 V bytes a row); two dozen instructions a logit make it a near thing.
+// A check misses by rounding when u falls within its error of p(x) / q(x), 1e-6 of it: fp32 weights do, and the first kernel waits for the logits (4 V
+// bytes a row).  A draw misses when u falls within the sums' error of any of 100 000 borders: with weights off by 2^-25 of themselves at
+// random, one draw in 10 000 (counted on rows of variance 6).  So the second kernel makes its weights to 2^-29: the argument as two fp32
+// numbers, a whole number R taken from it instead of the largest logit (exact, and chunks are joined by powers of
+// two), 2^y = 2^(n/16) 2^f with the sixteen powers kept in two parts and 2^f - 1, at most 1/32, from its series; its sums run in
+// fp64, and where a drafter's q is taken off it sums Z once more in the same way.
 #include <algorithm>
 #include <cmath>
-#include <type_traits>
 
 #include <cooperative_groups.h>
 
@@ -28,6 +26,7 @@ namespace cg = cooperative_groups;
 constexpr int VD_THREADS = 256;
 constexpr int VD_WARPS = VD_THREADS / 32;
 constexpr int VD_CHUNK = VD_THREADS * 8;          // logits of a chunk at the least, which sizes the workspace
+constexpr int VD_RESIDENT = 4;                    // blocks of the first kernel on an SM
 constexpr int VD_CLUSTER = 8;
 constexpr int VD_MAX_DRAFTS = 255;
 constexpr int VD_ROUND = 64;                      // steps of 128 logits that a block walks at a time
@@ -46,7 +45,8 @@ struct VerifyArgs {
     const int32_t *ids, *offsets;
     int batch, rows, V, chunks;
     float c_hi, c_lo;                             // log2(e) / temperature
-    double c;
+    double c, inv_c;
+    int chunk;                                    // logits of a chunk, whole steps of 1024
     const float* uniforms;
     int max_drafts;
     int32_t *accepted, *tokens;
@@ -88,24 +88,28 @@ struct VdWeights {
     const int2* s_pow;
     float c_hi, c_lo, s, least;                   // below `least` the weight is under 2^-120 of the largest, and 0
     int shift;                                    // -r, where an exponent stands
-    // The weight of l as hi + lo.  NaN and -inf have none.
-    __device__ __forceinline__ void operator()(float l, float& hi, float& lo) const {
-        constexpr float ROUND = 12582912.0f;      // 1.5 * 2^23
-        const float x = fmaxf(l, least) - s;
-        const float t = __fmul_rn(x, c_hi);
-        const float low = fmaf(x, c_lo, fmaf(x, c_hi, -t));
-        const float z = fmaf(t, 16.0f, ROUND), n = z - ROUND;             // the low bits of z are those of n
-        const float f = fmaf(n, -0.0625f, t) + low;
-        const int i = __float_as_int(z);
-        const int2 p = s_pow[i & 15];
-        const float g = fmaf(f, fmaf(f, fmaf(f, fmaf(f, 9.6181291e-3f, 5.5504109e-2f), 0.24022651f), 0.69314718f), __int_as_float(p.y));   // ln(2)^k / k!
-        hi = l >= least ? __int_as_float(p.x + (i << 19) + shift) : 0.0f;
-        lo = hi * g;
+    // The weights of two logits as hi + lo.  NaN and -inf have none.
+    __device__ __forceinline__ void operator()(float l0, float l1, float2& hi, float2& lo) const {
+        const f32x2 round = two(12582912.0f, 12582912.0f), less_round = two(-12582912.0f, -12582912.0f);      // 1.5 * 2^23
+        const f32x2 c = two(c_hi, c_hi), x = add2(two(fmaxf(l0, least), fmaxf(l1, least)), two(-s, -s));
+        const f32x2 t = mul2(x, c), low = fma2(x, two(c_lo, c_lo), fma2(x, c, mul2(x, two(-c_hi, -c_hi))));
+        const f32x2 z = fma2(t, two(16.0f, 16.0f), round), n = add2(z, less_round);      // the low bits of z are those of n
+        const f32x2 f = add2(fma2(n, two(-0.0625f, -0.0625f), t), low);
+        const float2 zz = each(z);
+        const int i0 = __float_as_int(zz.x), i1 = __float_as_int(zz.y);
+        const int2 p0 = s_pow[i0 & 15], p1 = s_pow[i1 & 15];
+        f32x2 g = fma2(f, two(9.6181291e-3f, 9.6181291e-3f), two(5.5504109e-2f, 5.5504109e-2f));              // ln(2)^k / k!
+        g = fma2(f, g, two(0.24022651f, 0.24022651f));
+        g = fma2(f, g, two(0.69314718f, 0.69314718f));
+        g = fma2(f, g, two(__int_as_float(p0.y), __int_as_float(p1.y)));
+        hi.x = l0 >= least ? __int_as_float(p0.x + (i0 << 19) + shift) : 0.0f;
+        hi.y = l1 >= least ? __int_as_float(p1.x + (i1 << 19) + shift) : 0.0f;
+        lo = each(mul2(two(hi.x, hi.y), g));
     }
 };
 __device__ __forceinline__ VdWeights vd_weights(const VerifyArgs& a, const int2* s_pow, float top) {
     const VdRef ref = vd_ref(a, top);
-    const float least = ref.s + (float)((double)(ref.r - 120) / a.c);
+    const float least = ref.s + (float)((double)(ref.r - 120) * a.inv_c);
     return VdWeights{s_pow, a.c_hi, a.c_lo, ref.s, fmaxf(least, -3.402823466e38f), (int)((unsigned)-ref.r << 23)};
 }
 
@@ -124,76 +128,87 @@ __device__ __forceinline__ VdBest vd_warp_best(VdBest a) {
     return a;
 }
 
-// grid (chunks, rows); EACH logits of a thread
-template <bool WIDE, bool GREEDY, int EACH>
+// grid (chunks, rows).  A thread takes sixteen logits of every 4096, the next ones under way, and adds them up relative to the largest of its
+// first; the threads' sums meet at the end.  (`top` of a part is then what its sum is relative to, no more than 60 / c below the largest.)
+template <bool WIDE, bool GREEDY>
 __global__ void __launch_bounds__(VD_THREADS) verify_stats_kernel(const __grid_constant__ VerifyArgs a) {
+    constexpr int HALF = 4 * VD_THREADS, EACH = 16, STEP = VD_THREADS * EACH;
     __shared__ VdPart s_part[VD_WARPS];
-    __shared__ int2 s_pow[16];
     asm volatile("griddepcontrol.launch_dependents;");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int live = a.offsets[a.batch];
-    bool table = false;
-    for (int row = blockIdx.y; row < a.rows; row += gridDim.y) {
-        if (row >= live) return;
+    const int live = min(a.offsets[a.batch], a.rows), c0 = blockIdx.x * a.chunk, c1 = min(a.V, c0 + a.chunk);
+    for (int row = blockIdx.y; row < live; row += gridDim.y) {
         const float* l = a.logits + row * a.ls;
-        const int c0 = blockIdx.x * (VD_THREADS * EACH);
-        float x[EACH];
-        VdBest best{-INFINITY, -1};
+        auto load = [&](int at, float (&x)[EACH]) {
 #pragma unroll
-        for (int i = 0; i < EACH; i += 4) {
-            const int at = c0 + i * VD_THREADS + 4 * threadIdx.x;
-            if (WIDE) {
-                const float4 f = at < a.V ? *reinterpret_cast<const float4*>(l + at) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-                x[i] = f.x; x[i + 1] = f.y; x[i + 2] = f.z; x[i + 3] = f.w;
-            } else {
+            for (int i = 0; i < EACH / 4; ++i) {
+                const int p = at + i * HALF;
+                if (WIDE) {
+                    const float4 f = p < c1 ? *reinterpret_cast<const float4*>(l + p) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                    x[4 * i] = f.x; x[4 * i + 1] = f.y; x[4 * i + 2] = f.z; x[4 * i + 3] = f.w;
+                } else {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) x[i + k] = at + k < a.V ? l[at + k] : -INFINITY;
+                    for (int k = 0; k < 4; ++k) x[4 * i + k] = p + k < c1 ? l[p + k] : -INFINITY;
+                }
             }
-        }
-        if (!GREEDY && !table) {
-            vd_table(s_pow);
-            table = true;
-        }
-        if (GREEDY) {
+        };
+        VdBest best{-INFINITY, -1};
+        float sum = 0.0f, s = 0.0f, less_r = 0.0f, least = 0.0f;
+        float limit = -INFINITY;                   // a weight of 2^60 is as good as one of 1: what sums are relative to changes once, as a rule
+        auto take = [&](int at, const float (&x)[EACH]) {
+            if (GREEDY) {
 #pragma unroll
-            for (int i = 0; i < EACH; ++i)
-                if (x[i] > best.v) best = VdBest{x[i], c0 + (i & ~3) * VD_THREADS + 4 * (int)threadIdx.x + (i & 3)};
-            best = vd_warp_best(best);
-        } else {                                   // where it stands is not asked
+                for (int i = 0; i < EACH; ++i)
+                    if (x[i] > best.v) best = VdBest{x[i], at + (i >> 2) * HALF + (i & 3)};
+                return;
+            }
+            float top = x[0];
 #pragma unroll
-            for (int i = 0; i < EACH; ++i) best.v = fmaxf(best.v, x[i]);
-            best.v = warp_max(best.v);
-            best.i = best.v > -INFINITY ? 0 : -1;
-        }
-        __syncthreads();                           // the table is there; the row before is done with s_part
-        double sum = 0.0;
-        if (!GREEDY && best.i >= 0) {
+            for (int i = 1; i < EACH; ++i) top = fmaxf(top, x[i]);
+            if (top > limit) {
+                sum *= (float)vd_rescale(a, best.v, top);
+                best = VdBest{top, 0};             // where it stands is not asked
+                const VdRef ref = vd_ref(a, top);
+                s = ref.s;
+                less_r = (float)-ref.r;
+                least = fmaxf(ref.s + (float)((double)(ref.r - 126) * a.inv_c), -3.402823466e38f);
+                limit = fminf(top + (float)(60.0 * a.inv_c), 3.402823466e38f);
+            }
             if (best.v == INFINITY) {              // infinite logits share the mass
 #pragma unroll
-                for (int i = 0; i < EACH; ++i) sum += x[i] == INFINITY ? 1.0 : 0.0;
-            } else {
-                const VdWeights weigh = vd_weights(a, s_pow, best.v);
-                float rest = 0.0f;
+                for (int i = 0; i < EACH; ++i) sum += x[i] == INFINITY ? 1.0f : 0.0f;
+            } else if (best.i >= 0) {
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int i = 0; i < EACH; ++i) {
-                    float hi, lo;
-                    weigh(x[i], hi, lo);
-                    sum += (double)hi;
-                    rest += lo;
+                for (int i = 0; i < EACH; ++i) {   // NaN and -inf count 2^-126
+                    float e;
+                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(fmaxf(x[i], least) - s, a.c_hi, less_r)));
+                    part[i & 3] += e;
                 }
-                sum += (double)rest;
+                sum += (part[0] + part[1]) + (part[2] + part[3]);
             }
-            sum = warp_sum_d(sum);
+        };
+        float x[EACH], y[EACH];
+        int at = c0 + 4 * threadIdx.x;
+        load(at, x);
+        for (; at < c1; at += 2 * STEP) {
+            load(at + STEP, y);
+            take(at, x);
+            load(at + 2 * STEP, x);
+            take(at + STEP, y);
         }
-        if (lane == 0) s_part[warp] = VdPart{sum, best.v, best.i};
+        const VdBest top = vd_warp_best(best);
+        double all = 0.0;
+        if (!GREEDY) all = warp_sum_d(best.i >= 0 ? (double)sum * vd_rescale(a, best.v, top.v) : 0.0);
+        if (lane == 0) s_part[warp] = VdPart{all, top.v, top.i};
         __syncthreads();
         if (warp == 0) {
             const VdPart p = s_part[lane % VD_WARPS];
             best = vd_warp_best(VdBest{p.top, p.at});
-            sum = !GREEDY && lane < VD_WARPS && p.at >= 0 ? p.sum * vd_rescale(a, p.top, best.v) : 0.0;
-            sum = warp_sum_d(sum);
-            if (lane == 0) a.part[(int64_t)row * a.chunks + blockIdx.x] = VdPart{sum, best.v, best.i};
+            if (!GREEDY) all = warp_sum_d(lane < VD_WARPS && p.at >= 0 ? p.sum * vd_rescale(a, p.top, best.v) : 0.0);
+            if (lane == 0) a.part[(int64_t)row * a.chunks + blockIdx.x] = VdPart{all, best.v, best.i};
         }
+        __syncthreads();                           // s_part is read
     }
 }
 
@@ -218,7 +233,7 @@ __global__ void __launch_bounds__(VD_THREADS) verify_pick_kernel(const __grid_co
     __shared__ bool s_keep[VD_MAX_DRAFTS + 1];
     __shared__ float s_top[VD_MAX_DRAFTS + 1];
     __shared__ int s_at[VD_MAX_DRAFTS + 1];
-    __shared__ double s_z[VD_MAX_DRAFTS + 1], s_mass[2][VD_WARPS];
+    __shared__ double s_mass[3][VD_WARPS];
     __shared__ int2 s_pow[16];
     __shared__ double s_step[VD_ROUND];
     cg::cluster_group cluster = cg::this_cluster();
@@ -248,14 +263,13 @@ __global__ void __launch_bounds__(VD_THREADS) verify_pick_kernel(const __grid_co
             if (GREEDY) {
                 keep = there && best.i == x;
             } else if (there && best.i >= 0) {
-                float hi = l == INFINITY ? 1.0f : 0.0f, lo = 0.0f;
-                if (best.v < INFINITY) vd_weights(a, s_pow, best.v)(l, hi, lo);
-                keep = (double)u * (double)q * z < (double)hi + (double)lo;
+                float2 hi = make_float2(l == INFINITY ? 1.0f : 0.0f, 0.0f), lo = make_float2(0.0f, 0.0f);
+                if (best.v < INFINITY) vd_weights(a, s_pow, best.v)(l, l, hi, lo);
+                keep = (double)u * (double)q * z < (double)hi.x + (double)lo.x;
             }
             s_keep[j] = keep;
             s_top[j] = best.v;
             s_at[j] = best.i;
-            s_z[j] = z;
         }
     }
     __syncthreads();
@@ -269,7 +283,7 @@ __global__ void __launch_bounds__(VD_THREADS) verify_pick_kernel(const __grid_co
         const float* q = refused && a.draft ? a.draft + row * a.ds : nullptr;
         const int without = refused && !a.draft ? a.ids[row + 1] : -1;
         const float top = s_top[n];
-        const double z = s_z[n];
+        double z = 0.0;
         const VdWeights weigh = vd_weights(a, s_pow, top);
         // segment of a warp: whole steps of 128 logits
         const int steps = ((a.V + 127) / 128 + VD_CLUSTER * VD_WARPS - 1) / (VD_CLUSTER * VD_WARPS), seg = steps * 128;
@@ -295,23 +309,37 @@ __global__ void __launch_bounds__(VD_THREADS) verify_pick_kernel(const __grid_co
             return f;
         };
         auto masses = [&](int at, const Four& f, bool from_p, double (&r)[4]) {
-            const float x[4] = {f.l.x, f.l.y, f.l.z, f.l.w}, y[4] = {f.q.x, f.q.y, f.q.z, f.q.w};
+            float2 h0, h1, r0, r1;
+            if (top < INFINITY) {
+                weigh(f.l.x, f.l.y, h0, r0);
+                weigh(f.l.z, f.l.w, h1, r1);
+            } else {
+                h0 = make_float2(f.l.x == INFINITY ? 1.0f : 0.0f, f.l.y == INFINITY ? 1.0f : 0.0f);
+                h1 = make_float2(f.l.z == INFINITY ? 1.0f : 0.0f, f.l.w == INFINITY ? 1.0f : 0.0f);
+                r0 = r1 = make_float2(0.0f, 0.0f);
+            }
+            r[0] = (double)h0.x + (double)r0.x;
+            r[1] = (double)h0.y + (double)r0.y;
+            r[2] = (double)h1.x + (double)r1.x;
+            r[3] = (double)h1.y + (double)r1.y;
+            if (from_p) return;
+            if (q) {
+                const float y[4] = {f.q.x, f.q.y, f.q.z, f.q.w};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                float hi = x[k] == INFINITY ? 1.0f : 0.0f, lo = 0.0f;
-                if (top < INFINITY) weigh(x[k], hi, lo);
-                r[k] = (double)hi + (double)lo;
-                if (!from_p && q) {
+                for (int k = 0; k < 4; ++k) {
                     r[k] = fma(-(double)y[k], z, r[k]);
                     if (!(r[k] > 0.0)) r[k] = 0.0;
                 }
-                if (!from_p && at + k == without) r[k] = 0.0;
+            } else if ((unsigned)(without - at) < 4u) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (at + k == without) r[k] = 0.0;
             }
         };
         const int own = (rank * VD_WARPS + warp) * seg;
-        bool from_p = !refused;
+        bool from_p = !refused || q;               // with a drafter's q, first Z: the mass of all of p
         double lane_from = 0.0, lane_mid = 0.0, lane_to = 0.0, total = 0.0;
-        for (int pass = 0; pass < 2; ++pass) {                // the second only where max(p - q, 0) has no mass
+        for (int pass = 0; pass < 3; ++pass) {
             double sum = 0.0;
             constexpr int AHEAD = 4;
             for (int s0 = 0; s0 < steps; s0 += AHEAD) {
@@ -349,8 +377,13 @@ __global__ void __launch_bounds__(VD_THREADS) verify_pick_kernel(const __grid_co
             lane_from = prev;
             lane_mid = mid;
             lane_to = upto;
+            if (pass == 0 && refused && q) {
+                z = total;
+                from_p = false;
+                continue;
+            }
             if (total > 0.0 || from_p) break;
-            from_p = true;
+            from_p = true;                         // max(p - q, 0) has no mass
         }
         const float u = a.uniforms[first + count - 1];
         const double mark = (u > 0.0f ? fmin((double)u, 1.0 - 1.0 / 16777216.0) : 0.0) * total;
@@ -448,28 +481,34 @@ int b200_verify_drafts(const float* logits, int64_t logits_stride, const float* 
     B200_REQUIRE(rows == 0 || (logits && ids && uniforms), "%s: null pointer", who);
     B200_REQUIRE(row_offsets && accepted && tokens && workspace, "%s: null pointer", who);
     B200_REQUIRE(logits_stride >= V && (!draft_probs || draft_stride >= V), "%s: a stride is shorter than its row", who);
-    B200_REQUIRE(temperature == temperature && temperature < INFINITY, "%s: the temperature must be a finite number", who);
+    B200_REQUIRE(temperature <= 1e30f, "%s: the temperature must be a number of at most 1e30", who);
     B200_REQUIRE(aligned16(workspace) && workspace_bytes >= need, "%s: the workspace must be 16-byte aligned and have %zu bytes", who, need);
     const bool greedy = temperature <= 0.0f;
     const double c = greedy ? 0.0 : 1.4426950408889634 / (double)temperature;
     const float hi = (float)c;
     B200_REQUIRE(hi < INFINITY, "%s: the temperature is too small", who);
     VerifyArgs a{logits, logits_stride, draft_probs, draft_stride, ids, row_offsets, batch, rows, V, 0,
-                 hi, (float)(c - (double)hi), c, uniforms, max_drafts, accepted, tokens, static_cast<VdPart*>(workspace)};
+                 hi, (float)(c - (double)hi), c, greedy ? 0.0 : 1.0 / c, 0, uniforms, max_drafts, accepted, tokens, static_cast<VdPart*>(workspace)};
     const bool wide = aligned16(logits) && V % 4 == 0 && logits_stride % 4 == 0 &&
                       (!draft_probs || (aligned16(draft_probs) && draft_stride % 4 == 0));
     const dim3 block(VD_THREADS);
     if (rows > 0) {
-        // chunks of 8192 where they fill the device: a quarter of the blocks' fixed costs; else of 2048
-        const bool many = (int64_t)rows * ceil_div(V, 4 * VD_CHUNK) >= 2 * num_sms();
-        a.chunks = ceil_div(V, many ? 4 * VD_CHUNK : VD_CHUNK);
+        // Chunks so that the rounds of blocks over the device, each as long as a chunk and what a block costs besides (about 3000 logits'
+        // worth), take the least; none of less than 2048 logits.
+        const int slots = VD_RESIDENT * num_sms(), most = ceil_div(V, VD_CHUNK);
+        int64_t least = INT64_MAX;
+        for (int n = 1; n <= std::min(most, 64); ++n) {
+            const int chunk = ceil_div(ceil_div(V, n), 1024) * 1024;
+            const int64_t cost = ceil_div64((int64_t)rows * ceil_div(V, chunk), slots) * (chunk + 3000);
+            if (cost < least) {
+                least = cost;
+                a.chunk = chunk;
+            }
+        }
+        a.chunks = ceil_div(V, a.chunk);
         const dim3 grid(a.chunks, std::min(rows, 65535));
-        auto pick = [&](auto each) {
-            constexpr int E = decltype(each)::value;
-            return wide ? (greedy ? verify_stats_kernel<true, true, E> : verify_stats_kernel<true, false, E>)
-                        : (greedy ? verify_stats_kernel<false, true, E> : verify_stats_kernel<false, false, E>);
-        };
-        auto kern = many ? pick(std::integral_constant<int, 32>()) : pick(std::integral_constant<int, 8>());
+        auto kern = wide ? (greedy ? verify_stats_kernel<true, true> : verify_stats_kernel<true, false>)
+                         : (greedy ? verify_stats_kernel<false, true> : verify_stats_kernel<false, false>);
         rc = launch_serve("verify_stats_kernel", kern, grid, block, 0, 1, false, a);
         if (rc) return rc;
     }
