@@ -26,7 +26,7 @@ namespace cg = cooperative_groups;
 constexpr int VD_THREADS = 256;
 constexpr int VD_WARPS = VD_THREADS / 32;
 constexpr int VD_CHUNK = VD_THREADS * 8;          // logits of a chunk at the least, which sizes the workspace
-constexpr int VD_RESIDENT = 4;                    // blocks of the first kernel on an SM
+constexpr int VD_RESIDENT = 4;                    // blocks on an SM (the second kernel's 64 x 8 all at once)
 constexpr int VD_CLUSTER = 8;
 constexpr int VD_MAX_DRAFTS = 255;
 constexpr int VD_ROUND = 64;                      // steps of 128 logits that a block walks at a time
@@ -88,7 +88,7 @@ struct VdWeights {
     const int2* s_pow;
     float c_hi, c_lo, s, least;                   // below `least` the weight is under 2^-120 of the largest, and 0
     int shift;                                    // -r, where an exponent stands
-    // The weights of two logits as hi + lo.  NaN and -inf have none.
+    // The weights of two logits as hi + lo, hi the sum's fp32 value.  NaN and -inf have none.
     __device__ __forceinline__ void operator()(float l0, float l1, float2& hi, float2& lo) const {
         const f32x2 round = two(12582912.0f, 12582912.0f), less_round = two(-12582912.0f, -12582912.0f);      // 1.5 * 2^23
         const f32x2 c = two(c_hi, c_hi), x = add2(two(fmaxf(l0, least), fmaxf(l1, least)), two(-s, -s));
@@ -102,9 +102,10 @@ struct VdWeights {
         g = fma2(f, g, two(0.24022651f, 0.24022651f));
         g = fma2(f, g, two(0.69314718f, 0.69314718f));
         g = fma2(f, g, two(__int_as_float(p0.y), __int_as_float(p1.y)));
-        hi.x = l0 >= least ? __int_as_float(p0.x + (i0 << 19) + shift) : 0.0f;
-        hi.y = l1 >= least ? __int_as_float(p1.x + (i1 << 19) + shift) : 0.0f;
-        lo = each(mul2(two(hi.x, hi.y), g));
+        const f32x2 p = two(l0 >= least ? __int_as_float(p0.x + (i0 << 19) + shift) : 0.0f, l1 >= least ? __int_as_float(p1.x + (i1 << 19) + shift) : 0.0f);
+        const f32x2 less = two(-1.0f, -1.0f), pg = mul2(p, g), sum = add2(p, pg);        // pg is at most p / 32
+        hi = each(sum);
+        lo = each(fma2(fma2(p, less, sum), less, pg));                                   // what rounding the sum cut off
     }
 };
 __device__ __forceinline__ VdWeights vd_weights(const VerifyArgs& a, const int2* s_pow, float top) {
@@ -131,7 +132,7 @@ __device__ __forceinline__ VdBest vd_warp_best(VdBest a) {
 // grid (chunks, rows).  A thread takes sixteen logits of every 4096, the next ones under way, and adds them up relative to the largest of its
 // first; the threads' sums meet at the end.  (`top` of a part is then what its sum is relative to, no more than 60 / c below the largest.)
 template <bool WIDE, bool GREEDY>
-__global__ void __launch_bounds__(VD_THREADS) verify_stats_kernel(const __grid_constant__ VerifyArgs a) {
+__global__ void __launch_bounds__(VD_THREADS, VD_RESIDENT) verify_stats_kernel(const __grid_constant__ VerifyArgs a) {
     constexpr int HALF = 4 * VD_THREADS, EACH = 16, STEP = VD_THREADS * EACH;
     __shared__ VdPart s_part[VD_WARPS];
     asm volatile("griddepcontrol.launch_dependents;");
@@ -229,7 +230,7 @@ __device__ __forceinline__ void vd_join(const VerifyArgs& a, int row, int lane, 
 
 // grid (8 per sequence); a cluster has a sequence
 template <bool WIDE, bool GREEDY>
-__global__ void __launch_bounds__(VD_THREADS) verify_pick_kernel(const __grid_constant__ VerifyArgs a) {
+__global__ void __launch_bounds__(VD_THREADS, VD_RESIDENT) verify_pick_kernel(const __grid_constant__ VerifyArgs a) {
     __shared__ bool s_keep[VD_MAX_DRAFTS + 1];
     __shared__ float s_top[VD_MAX_DRAFTS + 1];
     __shared__ int s_at[VD_MAX_DRAFTS + 1];
@@ -290,12 +291,12 @@ __global__ void __launch_bounds__(VD_THREADS) verify_pick_kernel(const __grid_co
         struct Four {
             float4 l, q;
         };
-        auto load = [&](int at) {
+        auto load = [&](int at, bool with_q) {
             Four f{make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY), make_float4(0.f, 0.f, 0.f, 0.f)};
             if (WIDE) {
                 if (at < a.V) {
                     f.l = __ldg(reinterpret_cast<const float4*>(l + at));
-                    if (q) f.q = __ldg(reinterpret_cast<const float4*>(q + at));
+                    if (with_q) f.q = __ldg(reinterpret_cast<const float4*>(q + at));
                 }
             } else {
                 float *x = &f.l.x, *y = &f.q.x;
@@ -303,25 +304,28 @@ __global__ void __launch_bounds__(VD_THREADS) verify_pick_kernel(const __grid_co
                 for (int k = 0; k < 4; ++k)
                     if (at + k < a.V) {
                         x[k] = l[at + k];
-                        if (q) y[k] = q[at + k];
+                        if (with_q) y[k] = q[at + k];
                     }
             }
             return f;
         };
-        auto masses = [&](int at, const Four& f, bool from_p, double (&r)[4]) {
-            float2 h0, h1, r0, r1;
+        auto weights = [&](const Four& f, float (&hi)[4], float (&lo)[4]) {
             if (top < INFINITY) {
+                float2 h0, h1, r0, r1;
                 weigh(f.l.x, f.l.y, h0, r0);
                 weigh(f.l.z, f.l.w, h1, r1);
-            } else {
-                h0 = make_float2(f.l.x == INFINITY ? 1.0f : 0.0f, f.l.y == INFINITY ? 1.0f : 0.0f);
-                h1 = make_float2(f.l.z == INFINITY ? 1.0f : 0.0f, f.l.w == INFINITY ? 1.0f : 0.0f);
-                r0 = r1 = make_float2(0.0f, 0.0f);
+                hi[0] = h0.x; hi[1] = h0.y; hi[2] = h1.x; hi[3] = h1.y;
+                lo[0] = r0.x; lo[1] = r0.y; lo[2] = r1.x; lo[3] = r1.y;
+            } else {                               // infinite logits share the mass
+                hi[0] = f.l.x == INFINITY; hi[1] = f.l.y == INFINITY; hi[2] = f.l.z == INFINITY; hi[3] = f.l.w == INFINITY;
+                lo[0] = lo[1] = lo[2] = lo[3] = 0.0f;
             }
-            r[0] = (double)h0.x + (double)r0.x;
-            r[1] = (double)h0.y + (double)r0.y;
-            r[2] = (double)h1.x + (double)r1.x;
-            r[3] = (double)h1.y + (double)r1.y;
+        };
+        auto masses = [&](int at, const Four& f, bool from_p, double (&r)[4]) {
+            float hi[4], lo[4];
+            weights(f, hi, lo);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) r[k] = (double)hi[k] + (double)lo[k];
             if (from_p) return;
             if (q) {
                 const float y[4] = {f.q.x, f.q.y, f.q.z, f.q.w};
@@ -341,19 +345,49 @@ __global__ void __launch_bounds__(VD_THREADS) verify_pick_kernel(const __grid_co
         double lane_from = 0.0, lane_mid = 0.0, lane_to = 0.0, total = 0.0;
         for (int pass = 0; pass < 3; ++pass) {
             double sum = 0.0;
-            constexpr int AHEAD = 4;
-            for (int s0 = 0; s0 < steps; s0 += AHEAD) {
-                Four f[AHEAD];
+            float rest = 0.0f;                     // what the weights' second parts come to, 2^-24 of the sum: in fp32
+            const bool with_q = !from_p && q;
+            auto add = [&](int at, const Four& f) {
+                float hi[4], lo[4];
+                weights(f, hi, lo);
+                if (with_q) {
+                    const float y[4] = {f.q.x, f.q.y, f.q.z, f.q.w};
 #pragma unroll
-                for (int s = 0; s < AHEAD; ++s) f[s] = load(s0 + s < steps ? own + (s0 + s) * 128 + 4 * lane : a.V);
-#pragma unroll
-                for (int s = 0; s < AHEAD; ++s) {
-                    if (s0 + s >= steps) break;
-                    double r[4];
-                    masses(own + (s0 + s) * 128 + 4 * lane, f[s], from_p, r);
-                    sum += (r[0] + r[1]) + (r[2] + r[3]);
+                    for (int k = 0; k < 4; ++k) {
+                        const double r = fma(-(double)y[k], z, (double)hi[k]);
+                        if (r > 0.0) {
+                            sum += r;
+                            rest += lo[k];
+                        }
+                    }
+                    return;
                 }
+                if (!from_p && (unsigned)(without - at) < 4u) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (at + k == without) hi[k] = lo[k] = 0.0f;
+                }
+                sum += ((double)hi[0] + (double)hi[1]) + ((double)hi[2] + (double)hi[3]);
+                rest += (lo[0] + lo[1]) + (lo[2] + lo[3]);
+            };
+            // two steps at a time, the next two under way
+            auto fetch = [&](int s, Four (&f)[2]) {
+                f[0] = load(s < steps ? own + s * 128 + 4 * lane : a.V, with_q);
+                f[1] = load(s + 1 < steps ? own + (s + 1) * 128 + 4 * lane : a.V, with_q);
+            };
+            auto take = [&](int s, const Four (&f)[2]) {
+                if (s < steps) add(own + s * 128 + 4 * lane, f[0]);
+                if (s + 1 < steps) add(own + (s + 1) * 128 + 4 * lane, f[1]);
+            };
+            Four u[2], v[2];
+            fetch(0, u);
+            for (int s = 0; s < steps; s += 4) {
+                fetch(s + 2, v);
+                take(s, u);
+                fetch(s + 4, u);
+                take(s + 2, v);
             }
+            sum += (double)rest;
             sum = warp_sum_d(sum);
             if (lane == 0) s_mass[pass][warp] = sum;
             cluster.sync();
@@ -401,7 +435,7 @@ __global__ void __launch_bounds__(VD_THREADS) verify_pick_kernel(const __grid_co
                 for (int s = warp; s < here; s += VD_WARPS) {
                     const int at = from + (s0 + s) * 128 + 4 * lane;
                     double r[4];
-                    masses(at, load(at), from_p, r);
+                    masses(at, load(at, !from_p && q), from_p, r);
                     const double sum = warp_sum_d((r[0] + r[1]) + (r[2] + r[3]));
                     if (lane == 0) s_step[s] = sum;
                 }
@@ -420,7 +454,7 @@ __global__ void __launch_bounds__(VD_THREADS) verify_pick_kernel(const __grid_co
             if (warp == 0) {
                 const int at = from + found * 128 + 4 * lane;
                 double r[4];
-                masses(at, load(at), from_p, r);
+                masses(at, load(at, !from_p && q), from_p, r);
                 const double sum = (r[0] + r[1]) + (r[2] + r[3]);
                 double incl = sum;
 #pragma unroll
