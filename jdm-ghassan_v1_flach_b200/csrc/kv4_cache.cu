@@ -6,16 +6,16 @@
 // value, because an infinite one would make a NaN of every code 0, and of every masked probability in the attention over these
 // pages.
 //
-// What bounds both: the fp32 rows (8 KV hd bytes a token), a quarter of that again for the pages' lines.  Eight lanes share a block of 32, each
-// with the four elements of one 16-bit word, so a warp reads 512 consecutive bytes and the block's statistics take three
-// shuffles.
-#include <type_traits>
-
+// What bounds both: the fp32 rows (8 KV hd bytes a token), a quarter of that again for the pages' lines, with about 70 and 25
+// instructions per 16 bytes of row.  Eight lanes share a token's row of one head: lane g has the four elements 4 g .. 4 g + 3 of each block
+// of 32, which is one 16-bit word per block, and those words lie side by side.  So a warp reads and writes whole lines of the row
+// and eight bytes a lane of the codes, and a block's statistics take three shuffles.
 #include "serve.cuh"
 
 namespace b200 {
 
-constexpr int KC_THREADS = 256;
+constexpr int KC_THREADS = 128;
+constexpr int KC_ITEMS = KC_THREADS / 8;         // rows of a head at a time
 
 struct Kv4Rows {
     const float *k_in = nullptr, *v_in = nullptr;
@@ -24,8 +24,8 @@ struct Kv4Rows {
     const int32_t* slots = nullptr;
     uint8_t* pages = nullptr;
     int64_t n = 0;
-    int num_slots = 0, page = 1, KV = 0, nb = 0;
-    FastDiv by_page, by_nb;
+    int num_slots = 0, page = 1, KV = 0;
+    FastDiv by_page, by_KV;
     Kv4Page part;
 };
 
@@ -37,128 +37,169 @@ int kv4_check(const char* who, int num_pages, int page, int KV, int hd, int kind
     return B200_OK;
 }
 
-// Where block `blk` (head * nb + b) of `slot` stands: its codes' 16-bit words (stride nb) and its scale.
-struct KcPlace {
-    uint16_t* word;
-    uint8_t* scale;
-};
-template <int KIND>
-__device__ __forceinline__ KcPlace kc_place(const Kv4Rows& a, int slot, int blk, bool v) {
-    const int pg = (int)a.by_page.div(slot), off = slot - pg * a.page;
-    const int h = (int)a.by_nb.div(blk), b = blk - h * a.nb;
-    uint8_t* base = a.pages + (int64_t)pg * a.part.bytes;
-    const int64_t row = (int64_t)h * a.page + off;
-    return {reinterpret_cast<uint16_t*>(base + (v ? a.part.v_code : 0) + row * (a.nb * 16)) + b,
-            base + (v ? a.part.v_scale : a.part.k_scale) + (row * a.nb + b) * (KIND == 1 ? 4 : 2)};
-}
-
 __device__ __forceinline__ uint32_t kc_half(float x) {      // to fp16, the largest value instead of an infinity
     return float_to_half_bits(fminf(fmaxf(x, -65504.0f), 65504.0f));
 }
+// Largest and smallest, NaN if one is.
+__device__ __forceinline__ float kc_max(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float kc_min(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// The nearest whole number to v >= 0, halves up, as the low bits: floor(v + 1/2), both steps rounded down, which never passes a whole
+// number that the exact sum has not reached.
+__device__ __forceinline__ int kc_nearest(float v) { return __float_as_int(__fadd_rd(__fadd_rd(v, 0.5f), 8388608.0f)); }
 
-// Rows of a thread: its loads are all under way before the first is used.  Few rows: one, so that they spread over the device.
-constexpr int KC_ROWS = 4;
+// A row of a head: its token, its head, and where its codes and scales stand in the pages (K's or V's); slot < 0: in none.
+template <int HD, int KIND>
+struct KcItem {
+    int64_t row;
+    int head, slot;
+    int64_t codes, scales;
+    __device__ __forceinline__ KcItem(const Kv4Rows& a, int64_t item, bool v) {
+        row = item < a.n * a.KV ? (int64_t)a.by_KV.div((uint32_t)item) : -1;
+        head = (int)(item - row * a.KV);
+        slot = row >= 0 ? a.slots[row] : -1;
+        if ((uint32_t)slot >= (uint32_t)a.num_slots) slot = -1;
+        const int s = max(slot, 0), pg = (int)a.by_page.div(s), off = s - pg * a.page;
+        const int64_t at = (int64_t)pg * a.part.bytes + (v ? a.part.v_code : 0), token = (int64_t)head * a.page + off;
+        codes = at + token * (HD / 2);
+        scales = at + a.part.k_scale + token * (HD / 32 * (KIND == 1 ? 4 : 2));          // V's parts follow as K's do
+    }
+};
 
-// blockIdx.y: 0 K, 1 V.  Eight lanes per block of 32 elements, ROWS rows one after another.
-template <int KIND, bool WIDE, int ROWS>
+// blockIdx.y: 0 K, 1 V
+template <int HD, int KIND, bool WIDE>
 __global__ void __launch_bounds__(KC_THREADS) kv4_store_kernel(const __grid_constant__ Kv4Rows a) {
+    constexpr int NB = HD / 32;
     const bool v = blockIdx.y != 0;
-    const float* src = v ? a.v_in : a.k_in;
-    const int64_t stride = v ? a.vs : a.ks, row0 = (int64_t)blockIdx.x * ROWS;
-    const int blocks = a.KV * a.nb, g = threadIdx.x & 7;
-    int slot[ROWS];
+    const int g = threadIdx.x & 7;
+    const KcItem<HD, KIND> it(a, (int64_t)blockIdx.x * KC_ITEMS + (threadIdx.x >> 3), v);
+    const float* src = (v ? a.v_in + it.row * a.vs : a.k_in + it.row * a.ks) + (int64_t)it.head * HD + 4 * g;
+    float x[NB][4];
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) slot[r] = row0 + r < a.n ? a.slots[row0 + r] : -1;
-    for (int blk = threadIdx.x >> 3; blk < (blocks + 3) / 4 * 4; blk += KC_THREADS / 8) {       // whole warps: four blocks each
-        float x[ROWS][4];
+    for (int b = 0; b < NB; ++b) {
+        x[b][0] = x[b][1] = x[b][2] = x[b][3] = 0.0f;
+        if (it.row < 0) continue;
+        if (WIDE) {
+            const float4 f = *reinterpret_cast<const float4*>(src + 32 * b);
+            x[b][0] = f.x; x[b][1] = f.y; x[b][2] = f.z; x[b][3] = f.w;
+        } else {
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) {
-            x[r][0] = x[r][1] = x[r][2] = x[r][3] = 0.0f;
-            if (row0 + r >= a.n || blk >= blocks) continue;
-            const float* p = src + (row0 + r) * stride + (int64_t)blk * 32 + 4 * g;
-            if (WIDE) {
-                const float4 f = *reinterpret_cast<const float4*>(p);
-                x[r][0] = f.x; x[r][1] = f.y; x[r][2] = f.z; x[r][3] = f.w;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[r][i] = p[i];
-            }
+            for (int i = 0; i < 4; ++i) x[b][i] = src[32 * b + i];
         }
+    }
+    float lo[NB], hi[NB];                                    // kind 0: hi of the magnitudes
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) {
-            bool bad = !(isfinite(x[r][0]) && isfinite(x[r][1]) && isfinite(x[r][2]) && isfinite(x[r][3]));
-            bad = (__ballot_sync(0xffffffffu, bad) & (0xFFu << (threadIdx.x & 24))) != 0;
-            uint32_t code = 0, scale;
-            if (KIND == 0) {
-                float top = fmaxf(fmaxf(fabsf(x[r][0]), fabsf(x[r][1])), fmaxf(fabsf(x[r][2]), fabsf(x[r][3])));
-#pragma unroll
-                for (int s = 1; s < 8; s <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-                const float d = __fdiv_rn(top, 8.0f), inv = d > 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) code |= (uint32_t)(min(max((int)roundf(__fmul_rn(x[r][i], inv)), -8), 7) + 8) << (4 * i);
-                scale = kc_half(d);
-                if (bad) { code = 0x8888u; scale = 0; }
-            } else {
-                float lo = fminf(fminf(x[r][0], x[r][1]), fminf(x[r][2], x[r][3])), hi = fmaxf(fmaxf(x[r][0], x[r][1]), fmaxf(x[r][2], x[r][3]));
-#pragma unroll
-                for (int s = 1; s < 8; s <<= 1) {
-                    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, s));
-                    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, s));
-                }
-                const float d = __fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f), inv = d > 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) code |= (uint32_t)min(max((int)roundf(__fmul_rn(__fsub_rn(x[r][i], lo), inv)), 0), 15) << (4 * i);
-                scale = kc_half(d) | (kc_half(lo) << 16);
-                if (bad) { code = 0; scale = 0; }
-            }
-            if (blk < blocks && (uint32_t)slot[r] < (uint32_t)a.num_slots) {
-                const KcPlace at = kc_place<KIND>(a, slot[r], blk, v);
-                at.word[g * a.nb] = (uint16_t)code;
-                if (g == 0) {
-                    if (KIND == 1) *reinterpret_cast<uint32_t*>(at.scale) = scale;
-                    else *reinterpret_cast<uint16_t*>(at.scale) = (uint16_t)scale;
-                }
-            }
+    for (int b = 0; b < NB; ++b) {
+        if (KIND == 1) {
+            lo[b] = kc_min(kc_min(x[b][0], x[b][1]), kc_min(x[b][2], x[b][3]));
+            hi[b] = kc_max(kc_max(x[b][0], x[b][1]), kc_max(x[b][2], x[b][3]));
+        } else {
+            hi[b] = kc_max(kc_max(fabsf(x[b][0]), fabsf(x[b][1])), kc_max(fabsf(x[b][2]), fabsf(x[b][3])));
         }
+    }
+#pragma unroll
+    for (int s = 1; s < 8; s <<= 1)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            hi[b] = kc_max(hi[b], __shfl_xor_sync(0xffffffffu, hi[b], s));
+            if (KIND == 1) lo[b] = kc_min(lo[b], __shfl_xor_sync(0xffffffffu, lo[b], s));
+        }
+    // each lane makes one block's scale and inverse, and has the others' from its neighbours
+    float my_hi = hi[0], my_lo = KIND == 1 ? lo[0] : 0.0f;
+#pragma unroll
+    for (int b = 1; b < NB; ++b)
+        if (g % NB == b) {
+            my_hi = hi[b];
+            my_lo = KIND == 1 ? lo[b] : 0.0f;
+        }
+    const float d = KIND == 1 ? __fmul_rn(__fsub_rn(my_hi, my_lo), 1.0f / 15.0f) : __fmul_rn(my_hi, 0.125f);
+    const bool sound = my_hi < INFINITY && my_lo > -INFINITY;
+    const float my_inv = !sound ? -1.0f : d > 0.0f ? __frcp_rn(d) : 0.0f;      // -1: the block is to be zero
+    uint32_t word[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        const float inv = __shfl_sync(0xffffffffu, my_inv, b, 8);
+        uint32_t code = 0;
+        if (inv >= 0.0f && inv < INFINITY) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (KIND == 1) {
+                    // at most 15 of them; above its low bits a number's exponent only reaches bits 24 and up.  hi - lo = inf: inv = 0
+                    const float y = __fmul_rn(__fsub_rn(x[b][i], lo[b]), inv);
+                    code += (uint32_t)kc_nearest(y == y ? y : 0.0f) << (4 * i);
+                } else {
+                    const float y = __fmul_rn(x[b][i], inv);
+                    const int n = kc_nearest(fabsf(y)) - 0x4B000000;              // 0 .. 8
+                    code += (uint32_t)(y < 0.0f ? 8 - n : min(8 + n, 15)) << (4 * i);
+                }
+            }
+        } else if (KIND == 0) {
+            code = 0x8888u;
+        }
+        if (inv == INFINITY) {                               // a block of denormals: all that is not its zero (or minimum) is as far as codes go
+            code = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) code |= (KIND == 1 ? (x[b][i] > lo[b] ? 15u : 0u) : x[b][i] > 0.0f ? 15u : x[b][i] < 0.0f ? 0u : 8u) << (4 * i);
+        }
+        word[b] = code & 0xFFFFu;
+    }
+    if (it.slot < 0) return;
+    uint8_t* codes = a.pages + it.codes + g * (2 * NB);
+    if (NB == 4) *reinterpret_cast<uint2*>(codes) = make_uint2(word[0] | (word[1] << 16), word[NB > 2 ? 2 : 0] | (word[NB > 2 ? 3 : 0] << 16));
+    else *reinterpret_cast<uint32_t*>(codes) = word[0] | (word[1] << 16);
+    if (g < NB) {
+        uint8_t* scale = a.pages + it.scales + g * (KIND == 1 ? 4 : 2);
+        const float m = sound ? my_lo : 0.0f;
+        if (KIND == 1) *reinterpret_cast<uint32_t*>(scale) = sound ? kc_half(d) | (kc_half(m) << 16) : 0u;
+        else *reinterpret_cast<uint16_t*>(scale) = sound ? (uint16_t)kc_half(d) : (uint16_t)0;
     }
 }
 
-template <int KIND, bool WIDE, int ROWS>
+template <int HD, int KIND, bool WIDE>
 __global__ void __launch_bounds__(KC_THREADS) kv4_fetch_kernel(const __grid_constant__ Kv4Rows a) {
+    constexpr int NB = HD / 32;
     const bool v = a.k_out ? blockIdx.y != 0 : true;
-    float* dst = v ? a.v_out : a.k_out;
-    const int64_t stride = v ? a.vs : a.ks, row0 = (int64_t)blockIdx.x * ROWS;
-    const int words = a.KV * a.nb * 8;
-    int slot[ROWS];
-#pragma unroll
-    for (int r = 0; r < ROWS; ++r) slot[r] = row0 + r < a.n ? a.slots[row0 + r] : -1;
-    for (int w = threadIdx.x; w < words; w += KC_THREADS) {
-        uint32_t code[ROWS], scale[ROWS];
-#pragma unroll
-        for (int r = 0; r < ROWS; ++r) {
-            code[r] = scale[r] = 0;
-            if ((uint32_t)slot[r] >= (uint32_t)a.num_slots) continue;
-            const KcPlace at = kc_place<KIND>(a, slot[r], w >> 3, v);
-            code[r] = at.word[(w & 7) * a.nb];
-            scale[r] = KIND == 1 ? *reinterpret_cast<const uint32_t*>(at.scale) : *reinterpret_cast<const uint16_t*>(at.scale);
+    const int g = threadIdx.x & 7;
+    const KcItem<HD, KIND> it(a, (int64_t)blockIdx.x * KC_ITEMS + (threadIdx.x >> 3), v);
+    if (it.slot < 0) return;
+    uint32_t word[NB / 2], scale[KIND == 1 ? NB : NB / 2];
+    auto fill = [](uint32_t* w, int n, const uint8_t* p) {
+        if (n == 4) {
+            const uint4 f = *reinterpret_cast<const uint4*>(p);
+            w[0] = f.x; w[1] = f.y; w[2] = f.z; w[3] = f.w;
+        } else if (n == 2) {
+            const uint2 f = *reinterpret_cast<const uint2*>(p);
+            w[0] = f.x; w[1] = f.y;
+        } else {
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
         }
+    };
+    fill(word, NB / 2, a.pages + it.codes + g * (2 * NB));
+    fill(scale, KIND == 1 ? NB : NB / 2, a.pages + it.scales);
+    float* dst = (v ? a.v_out + it.row * a.vs : a.k_out + it.row * a.ks) + (int64_t)it.head * HD + 4 * g;
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) {
-            if ((uint32_t)slot[r] >= (uint32_t)a.num_slots) continue;
-            const float d = half_bits_to_float((uint16_t)scale[r]), m = half_bits_to_float((uint16_t)(scale[r] >> 16));
-            float x[4];
+    for (int b = 0; b < NB; ++b) {
+        const uint32_t code = word[b / 2] >> (b & 1 ? 16 : 0);
+        const uint32_t s = KIND == 1 ? scale[b < NB && KIND == 1 ? b : 0] : scale[b / 2] >> (b & 1 ? 16 : 0);
+        const float d = half_bits_to_float((uint16_t)s), m = KIND == 1 ? half_bits_to_float((uint16_t)(s >> 16)) : 0.0f;
+        float x[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int c = (code[r] >> (4 * i)) & 15;
-                x[i] = KIND == 1 ? __fadd_rn(__fmul_rn(d, (float)c), m) : __fmul_rn(d, (float)(c - 8));
-            }
-            float* p = dst + (row0 + r) * stride + (int64_t)w * 4;
-            if (WIDE) {
-                *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-            } else {
+        for (int i = 0; i < 4; ++i) {                       // a code under the exponent of 2^23 is 2^23 and itself
+            const float f = __int_as_float(((code >> (4 * i)) & 15) | 0x4B000000);
+            x[i] = KIND == 1 ? fmaf(d, f - 8388608.0f, m) : d * (f - 8388616.0f);       // d * code is exact: one rounding
+        }
+        if (WIDE) {
+            *reinterpret_cast<float4*>(dst + 32 * b) = make_float4(x[0], x[1], x[2], x[3]);
+        } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) p[i] = x[i];
-            }
+            for (int i = 0; i < 4; ++i) dst[32 * b + i] = x[i];
         }
     }
 }
@@ -168,9 +209,8 @@ static void kc_geometry(Kv4Rows& a, void* pages, int num_pages, int page, int KV
     a.num_slots = num_pages * page;
     a.page = page;
     a.KV = KV;
-    a.nb = hd / 32;
     a.by_page = FastDiv(page);
-    a.by_nb = FastDiv(a.nb);
+    a.by_KV = FastDiv(KV);
     a.part = Kv4Page(page, KV, hd, kind);
 }
 
@@ -193,7 +233,7 @@ int b200_kv4_store(const float* k, const float* v, int64_t k_stride, int64_t v_s
     if (n <= 0) return B200_OK;
     int rc = kv4_check("kv4_store", num_pages, page, KV, hd, kind);
     if (rc) return rc;
-    B200_REQUIRE(n <= 0x7fffffff, "kv4_store: too many rows");
+    B200_REQUIRE(n <= 0x7fffffff / KV, "kv4_store: too many rows");
     B200_REQUIRE(k && v && slots && pages, "kv4_store: null pointer");
     B200_REQUIRE(aligned16(pages), "kv4_store: pages must be 16-byte aligned");
     B200_REQUIRE(k_stride >= (int64_t)KV * hd && v_stride >= (int64_t)KV * hd, "kv4_store: a stride is shorter than its row");
@@ -201,14 +241,11 @@ int b200_kv4_store(const float* k, const float* v, int64_t k_stride, int64_t v_s
     kc_geometry(a, pages, num_pages, page, KV, hd, kind);
     a.k_in = k; a.v_in = v; a.ks = k_stride; a.vs = v_stride; a.slots = slots; a.n = n;
     const bool wide = aligned16(k) && aligned16(v) && k_stride % 4 == 0 && v_stride % 4 == 0;
-    const bool many = n >= KC_ROWS * num_sms();
-    const dim3 grid((unsigned)(many ? ceil_div64(n, KC_ROWS) : n), 2), block(KC_THREADS);
-    auto pick = [&](auto rows) {
-        constexpr int R = decltype(rows)::value;
-        return kind == 1 ? (wide ? kv4_store_kernel<1, true, R> : kv4_store_kernel<1, false, R>)
-                         : (wide ? kv4_store_kernel<0, true, R> : kv4_store_kernel<0, false, R>);
-    };
-    auto kern = many ? pick(std::integral_constant<int, KC_ROWS>()) : pick(std::integral_constant<int, 1>());
+    const dim3 grid((unsigned)ceil_div64(n * KV, KC_ITEMS), 2), block(KC_THREADS);
+    auto kern = hd == 64 ? (kind == 1 ? (wide ? kv4_store_kernel<64, 1, true> : kv4_store_kernel<64, 1, false>)
+                                      : (wide ? kv4_store_kernel<64, 0, true> : kv4_store_kernel<64, 0, false>))
+                         : (kind == 1 ? (wide ? kv4_store_kernel<128, 1, true> : kv4_store_kernel<128, 1, false>)
+                                      : (wide ? kv4_store_kernel<128, 0, true> : kv4_store_kernel<128, 0, false>));
     return launch_serve("kv4_store_kernel", kern, grid, block, 0, 1, false, a);
 }
 
@@ -217,7 +254,7 @@ int b200_kv4_fetch(const void* pages, int num_pages, int page, const int32_t* sl
     if (n <= 0) return B200_OK;
     int rc = kv4_check("kv4_fetch", num_pages, page, KV, hd, kind);
     if (rc) return rc;
-    B200_REQUIRE(n <= 0x7fffffff, "kv4_fetch: too many rows");
+    B200_REQUIRE(n <= 0x7fffffff / KV, "kv4_fetch: too many rows");
     B200_REQUIRE((k || v) && slots && pages, "kv4_fetch: null pointer");
     B200_REQUIRE(aligned16(pages), "kv4_fetch: pages must be 16-byte aligned");
     B200_REQUIRE((!k || k_stride >= (int64_t)KV * hd) && (!v || v_stride >= (int64_t)KV * hd), "kv4_fetch: a stride is shorter than its row");
@@ -225,14 +262,11 @@ int b200_kv4_fetch(const void* pages, int num_pages, int page, const int32_t* sl
     kc_geometry(a, const_cast<void*>(pages), num_pages, page, KV, hd, kind);
     a.k_out = k; a.v_out = v; a.ks = k_stride; a.vs = v_stride; a.slots = slots; a.n = n;
     const bool wide = (!k || (aligned16(k) && k_stride % 4 == 0)) && (!v || (aligned16(v) && v_stride % 4 == 0));
-    const bool many = n >= KC_ROWS * num_sms();
-    const dim3 grid((unsigned)(many ? ceil_div64(n, KC_ROWS) : n), k && v ? 2 : 1), block(KC_THREADS);
-    auto pick = [&](auto rows) {
-        constexpr int R = decltype(rows)::value;
-        return kind == 1 ? (wide ? kv4_fetch_kernel<1, true, R> : kv4_fetch_kernel<1, false, R>)
-                         : (wide ? kv4_fetch_kernel<0, true, R> : kv4_fetch_kernel<0, false, R>);
-    };
-    auto kern = many ? pick(std::integral_constant<int, KC_ROWS>()) : pick(std::integral_constant<int, 1>());
+    const dim3 grid((unsigned)ceil_div64(n * KV, KC_ITEMS), k && v ? 2 : 1), block(KC_THREADS);
+    auto kern = hd == 64 ? (kind == 1 ? (wide ? kv4_fetch_kernel<64, 1, true> : kv4_fetch_kernel<64, 1, false>)
+                                      : (wide ? kv4_fetch_kernel<64, 0, true> : kv4_fetch_kernel<64, 0, false>))
+                         : (kind == 1 ? (wide ? kv4_fetch_kernel<128, 1, true> : kv4_fetch_kernel<128, 1, false>)
+                                      : (wide ? kv4_fetch_kernel<128, 0, true> : kv4_fetch_kernel<128, 0, false>));
     return launch_serve("kv4_fetch_kernel", kern, grid, block, 0, 1, false, a);
 }
 
