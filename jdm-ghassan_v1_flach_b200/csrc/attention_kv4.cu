@@ -57,7 +57,7 @@ struct Kv4AttnArgs {
     Kv4Page part;
     float scale;
     int window;
-    int pairs;                                   // of a tile
+    int pairs, workers;                          // pairs of a tile; warps of the grid
     float* piece;                                // [2 * workers][pairs][hd + 4]: o, m, l of cut items
     struct A4Item* item;                         // [workers]
 };
@@ -98,7 +98,6 @@ __device__ __forceinline__ float a4_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ uint32_t a4_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 template <int BYTES>
 __device__ __forceinline__ void a4_copy(uint32_t dst, const uint8_t* src) {
     if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -187,7 +186,8 @@ __global__ void __launch_bounds__(A4_THREADS, A4_RESIDENT) attn_kv4_kernel(const
     extern __shared__ __align__(128) uint8_t a4_ring[];
     __shared__ int64_t s_sum[A4_WARPS], s_from[A4_THREADS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    asm volatile("griddepcontrol.launch_dependents;");
+    pdl_launch_dependents();
+    pdl_wait();
 
     // ---- this worker's share of the units ----
     const int share = (a.batch + A4_THREADS - 1) / A4_THREADS;
@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(A4_THREADS, A4_RESIDENT) attn_kv4_kernel(const
     constexpr bool Q_SHARED = NT > 1;
     uint8_t* ring = a4_ring + warp * RING;
     uint4(*s_q)[32] = reinterpret_cast<uint4(*)[32]>(a4_ring + A4_WARPS * RING + warp * a4_query_bytes(HD, NT));
-    const uint32_t ring_at = a4_smem(ring);
+    const uint32_t ring_at = smem_u32(ring);
 
     while (true) {
         const int weight = seq.units + A4_ITEM;
@@ -623,71 +623,81 @@ __global__ void __launch_bounds__(A4_THREADS, A4_RESIDENT) attn_kv4_kernel(const
     }
 }
 
-// Items that a worker began and others went on with: one block each, a thread per four dims of a pair, eight pieces at a time; what threads
-// that leaves take every other piece.
-constexpr int A4_JOIN = 256;
-
-template <int HD>
-__global__ void __launch_bounds__(A4_JOIN) attn_kv4_join_kernel(const __grid_constant__ Kv4AttnArgs a) {
-    constexpr int AT_ONCE = 8;
-    __shared__ float4 s_o[A4_JOIN];
-    __shared__ float2 s_ml[A4_JOIN];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const A4Item it = a.item[blockIdx.x];
-    if (it.more == 0) return;
-    const int columns = a.pairs * (HD / 4), groups = A4_JOIN / columns, group = threadIdx.x / columns;
-    const int col = threadIdx.x % columns, p = col / (HD / 4), c = col % (HD / 4) * 4;
-    // piece i: the worker's own second slot, then the first slots of those behind it
-    const float* mine = a.piece + ((int64_t)(2 * blockIdx.x) * a.pairs + p) * (HD + 4);
-    float mm = -INFINITY, ll = 0.0f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i0 = group; i0 <= it.more; i0 += AT_ONCE * groups) {
-        float2 ml[AT_ONCE];
-        float4 v[AT_ONCE];
+// Items that a worker began and others went on with, a block each: a thread per four dims of a pair and group of pieces, AT_ONCE pieces at
+// a time.  Many items have few pieces: a block with a thread per column or two.  Few items, that is few sequences, have many.
+template <int HD, int THREADS, int AT_ONCE>
+__global__ void __launch_bounds__(THREADS) attn_kv4_join_kernel(const __grid_constant__ Kv4AttnArgs a) {
+    __shared__ float4 s_o[THREADS];
+    __shared__ float2 s_ml[THREADS];
+    const int columns = a.pairs * (HD / 4), groups = THREADS / columns, lane = threadIdx.x & 31;
+    pdl_wait();
+    const int mine = blockIdx.x + lane * gridDim.x;              // the workers of this block
+    unsigned left = __ballot_sync(0xffffffffu, mine < a.workers && __ldcg(&a.item[min(mine, a.workers - 1)].more) > 0);
+    for (; left; left &= left - 1) {
+        const int worker = blockIdx.x + (__ffs(left) - 1) * gridDim.x;
+        const A4Item it = a.item[worker];
+        const int group = threadIdx.x / columns, col = threadIdx.x % columns, p = col / (HD / 4), c = col % (HD / 4) * 4;
+        // piece i: the worker's own second slot, then the first slots of those behind it
+        const float* pieces = a.piece + ((int64_t)(2 * worker) * a.pairs + p) * (HD + 4);
+        float mm = -INFINITY, ll = 0.0f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i0 = group; i0 <= it.more; i0 += AT_ONCE * groups) {
+            float2 ml[AT_ONCE];
+            float4 v[AT_ONCE];
 #pragma unroll
-        for (int k = 0; k < AT_ONCE; ++k) {
-            const int i = i0 + k * groups;
-            ml[k] = make_float2(-INFINITY, 0.0f);
-            v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (i <= it.more) {
-                const float* s = mine + (int64_t)(2 * i + (i == 0)) * a.pairs * (HD + 4);
-                ml[k] = __ldcg(reinterpret_cast<const float2*>(s + HD));
-                v[k] = __ldcg(reinterpret_cast<const float4*>(s + c));
+            for (int k = 0; k < AT_ONCE; ++k) {
+                const int i = i0 + k * groups;
+                ml[k] = make_float2(-INFINITY, 0.0f);
+                v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (i <= it.more) {
+                    const float* s = pieces + (int64_t)(2 * i + (i == 0)) * a.pairs * (HD + 4);
+                    ml[k] = __ldcg(reinterpret_cast<const float2*>(s + HD));
+                    v[k] = __ldcg(reinterpret_cast<const float4*>(s + c));
+                }
             }
-        }
-        float top = mm;
+            float top = mm;
 #pragma unroll
-        for (int k = 0; k < AT_ONCE; ++k) top = fmaxf(top, ml[k].x);
-        const float base = top == -INFINITY ? 0.0f : top, old = a4_exp2(mm - base);
-        ll *= old;
-        acc.x *= old; acc.y *= old; acc.z *= old; acc.w *= old;
+            for (int k = 0; k < AT_ONCE; ++k) top = fmaxf(top, ml[k].x);
+            const float base = top == -INFINITY ? 0.0f : top, old = a4_exp2(mm - base);
+            ll *= old;
+            acc.x *= old; acc.y *= old; acc.z *= old; acc.w *= old;
 #pragma unroll
-        for (int k = 0; k < AT_ONCE; ++k) {
-            const float f = a4_exp2(ml[k].x - base);
-            ll = fmaf(ml[k].y, f, ll);
-            acc.x = fmaf(v[k].x, f, acc.x); acc.y = fmaf(v[k].y, f, acc.y); acc.z = fmaf(v[k].z, f, acc.z); acc.w = fmaf(v[k].w, f, acc.w);
-        }
-        mm = top;
-    }
-    if (groups > 1) {
-        s_o[threadIdx.x] = acc;
-        s_ml[threadIdx.x] = make_float2(mm, ll);
-        __syncthreads();
-        if (group != 0) return;
-        for (int i = 1; i < groups; ++i) {
-            const float2 ml = s_ml[i * columns + threadIdx.x];
-            const float4 v = s_o[i * columns + threadIdx.x];
-            const float top = fmaxf(mm, ml.x), base = top == -INFINITY ? 0.0f : top, f0 = a4_exp2(mm - base), f1 = a4_exp2(ml.x - base);
-            ll = ll * f0 + ml.y * f1;
-            acc.x = acc.x * f0 + v.x * f1; acc.y = acc.y * f0 + v.y * f1; acc.z = acc.z * f0 + v.z * f1; acc.w = acc.w * f0 + v.w * f1;
+            for (int k = 0; k < AT_ONCE; ++k) {
+                const float f = a4_exp2(ml[k].x - base);
+                ll = fmaf(ml[k].y, f, ll);
+                acc.x = fmaf(v[k].x, f, acc.x); acc.y = fmaf(v[k].y, f, acc.y); acc.z = fmaf(v[k].z, f, acc.z); acc.w = fmaf(v[k].w, f, acc.w);
+            }
             mm = top;
         }
+        if (groups > 1) {
+            __syncthreads();                                 // the item before is read
+            s_o[threadIdx.x] = acc;
+            s_ml[threadIdx.x] = make_float2(mm, ll);
+            __syncthreads();
+            if (group == 0)
+                for (int i = 1; i < groups; ++i) {
+                    const float2 ml = s_ml[i * columns + threadIdx.x];
+                    const float4 v = s_o[i * columns + threadIdx.x];
+                    const float top = fmaxf(mm, ml.x), base = top == -INFINITY ? 0.0f : top, f0 = a4_exp2(mm - base), f1 = a4_exp2(ml.x - base);
+                    ll = ll * f0 + ml.y * f1;
+                    acc.x = acc.x * f0 + v.x * f1; acc.y = acc.y * f0 + v.y * f1; acc.z = acc.z * f0 + v.z * f1; acc.w = acc.w * f0 + v.w * f1;
+                    mm = top;
+                }
+        }
+        if (group == 0 && p < it.live) {
+            const int row = (int)a.by_group.div(it.pair + p);
+            const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+            float* dst = a.out + (int64_t)(it.first + row) * a.os + ((int64_t)it.kv * a.group + (it.pair + p - row * a.group)) * HD + c;
+            *reinterpret_cast<float4*>(dst) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+        }
     }
-    if (p >= it.live) return;
-    const int row = (int)a.by_group.div(it.pair + p);
-    const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-    float* dst = a.out + (int64_t)(it.first + row) * a.os + ((int64_t)it.kv * a.group + (it.pair + p - row * a.group)) * HD + c;
-    *reinterpret_cast<float4*>(dst) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+}
+
+template <int HD>
+static int launch_a4_join(const Kv4AttnArgs& a, int items) {
+    constexpr int THREADS = 2 * HD, AT_ONCE = HD / 16;
+    if (items > num_sms()) return launch_serve("attn_kv4_join_kernel", attn_kv4_join_kernel<HD, THREADS, AT_ONCE>, dim3(a.workers), dim3(THREADS), 0, 1, true, a);
+    return launch_serve("attn_kv4_join_kernel", attn_kv4_join_kernel<HD, 512, 8>, dim3(num_sms()), dim3(512), 0, 1, true, a);
 }
 
 // Tiles of four pairs that a warp takes at once, from the most pairs that a sequence has for a KV head.
@@ -699,7 +709,7 @@ static int launch_a4(const Kv4AttnArgs& a, int blocks) {
     auto kern = attn_kv4_kernel<HD, KIND, NT>;
     constexpr int smem = A4_WARPS * (a4_stages(NT) * A4Stage<HD, KIND>::BYTES + a4_query_bytes(HD, NT));
     if (smem > 48 * 1024) B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    return launch_serve("attn_kv4_kernel", kern, dim3(blocks), dim3(A4_THREADS), smem, 1, false, a);
+    return launch_serve("attn_kv4_kernel", kern, dim3(blocks), dim3(A4_THREADS), smem, 1, true, a);
 }
 
 }  // namespace b200
@@ -738,7 +748,7 @@ int b200_attention_paged_kv4(const float* q, int64_t q_stride, const int32_t* ro
     B200_REQUIRE(workspace_bytes >= need, "%s: the workspace has %zu bytes of %zu", who, workspace_bytes, need);
     const int nt = a4_tiles((int64_t)max_rows * (H / KV)), blocks = a4_blocks(), workers = blocks * A4_WARPS;
     Kv4AttnArgs a{q, q_stride, row_offsets, static_cast<const uint8_t*>(pages), num_pages, page_table, seq_lens, out, out_stride, batch,
-                  max_pages, page, H, KV, H / KV, FastDiv(page), FastDiv(H / KV), FastDiv(4 * nt), Kv4Page(page, KV, hd, kind), scale, window, 4 * nt,
+                  max_pages, page, H, KV, H / KV, FastDiv(page), FastDiv(H / KV), FastDiv(4 * nt), Kv4Page(page, KV, hd, kind), scale, window, 4 * nt, workers,
                   reinterpret_cast<float*>(static_cast<A4Item*>(workspace) + workers), static_cast<A4Item*>(workspace)};
     if (hd == 64)
         rc = kind == 1 ? (nt == 1 ? launch_a4<64, 1, 1>(a, blocks) : launch_a4<64, 1, 2>(a, blocks))
@@ -747,9 +757,8 @@ int b200_attention_paged_kv4(const float* q, int64_t q_stride, const int32_t* ro
         rc = kind == 1 ? (nt == 1 ? launch_a4<128, 1, 1>(a, blocks) : launch_a4<128, 1, 2>(a, blocks))
                        : (nt == 1 ? launch_a4<128, 0, 1>(a, blocks) : launch_a4<128, 0, 2>(a, blocks));
     if (rc) return rc;
-    const dim3 grid(workers);
-    return hd == 64 ? launch_serve("attn_kv4_join_kernel", attn_kv4_join_kernel<64>, grid, dim3(A4_JOIN), 0, 1, true, a)
-                    : launch_serve("attn_kv4_join_kernel", attn_kv4_join_kernel<128>, grid, dim3(A4_JOIN), 0, 1, true, a);
+    const int64_t items = (int64_t)batch * KV * (((int64_t)max_rows * (H / KV) + a.pairs - 1) / a.pairs);       // at the most
+    return hd == 64 ? launch_a4_join<64>(a, (int)std::min<int64_t>(items, 1 << 30)) : launch_a4_join<128>(a, (int)std::min<int64_t>(items, 1 << 30));
 }
 
 }  // extern "C"

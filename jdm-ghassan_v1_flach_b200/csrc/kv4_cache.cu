@@ -79,6 +79,7 @@ __global__ void __launch_bounds__(KC_THREADS) kv4_store_kernel(const __grid_cons
     constexpr int NB = HD / 32;
     const bool v = blockIdx.y != 0;
     const int g = threadIdx.x & 7;
+    short_begin();
     const KcItem<HD, KIND> it(a, (int64_t)blockIdx.x * KC_ITEMS + (threadIdx.x >> 3), v);
     const float* src = (v ? a.v_in + it.row * a.vs : a.k_in + it.row * a.ks) + (int64_t)it.head * HD + 4 * g;
     float x[NB][4];
@@ -167,6 +168,7 @@ __global__ void __launch_bounds__(KC_THREADS) kv4_fetch_kernel(const __grid_cons
     constexpr int NB = HD / 32;
     const bool v = a.k_out ? blockIdx.y != 0 : true;
     const int g = threadIdx.x & 7;
+    short_begin();
     const KcItem<HD, KIND> it(a, (int64_t)blockIdx.x * KC_ITEMS + (threadIdx.x >> 3), v);
     if (it.slot < 0) return;
     uint32_t word[NB / 2], scale[KIND == 1 ? NB : NB / 2];
@@ -246,7 +248,7 @@ int b200_kv4_store(const float* k, const float* v, int64_t k_stride, int64_t v_s
                                       : (wide ? kv4_store_kernel<64, 0, true> : kv4_store_kernel<64, 0, false>))
                          : (kind == 1 ? (wide ? kv4_store_kernel<128, 1, true> : kv4_store_kernel<128, 1, false>)
                                       : (wide ? kv4_store_kernel<128, 0, true> : kv4_store_kernel<128, 0, false>));
-    return launch_serve("kv4_store_kernel", kern, grid, block, 0, 1, false, a);
+    return launch_serve("kv4_store_kernel", kern, grid, block, 0, 1, short_grid(grid), a);
 }
 
 int b200_kv4_fetch(const void* pages, int num_pages, int page, const int32_t* slots, int64_t n, float* k, float* v,
@@ -267,7 +269,7 @@ int b200_kv4_fetch(const void* pages, int num_pages, int page, const int32_t* sl
                                       : (wide ? kv4_fetch_kernel<64, 0, true> : kv4_fetch_kernel<64, 0, false>))
                          : (kind == 1 ? (wide ? kv4_fetch_kernel<128, 1, true> : kv4_fetch_kernel<128, 1, false>)
                                       : (wide ? kv4_fetch_kernel<128, 0, true> : kv4_fetch_kernel<128, 0, false>));
-    return launch_serve("kv4_fetch_kernel", kern, grid, block, 0, 1, false, a);
+    return launch_serve("kv4_fetch_kernel", kern, grid, block, 0, 1, short_grid(grid), a);
 }
 
 }  // extern "C"

@@ -50,6 +50,7 @@ __global__ void __launch_bounds__(PP_THREADS) paged_plan_kernel(const __grid_con
     __shared__ long long s_part[PP_THREADS / 32][3];
     __shared__ int s_most[2], s_refused;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    short_begin();
     const long long head = a.at[0], tail = a.at[1];
     const bool sound = head >= 0 && tail >= head && tail - head <= (long long)a.ring_size;
     const long long avail = sound ? tail - head : 0;
@@ -211,9 +212,9 @@ extern "C" int b200_paged_plan(const int32_t* ctx_lens, const int32_t* new_lens,
                ring_at, ring_at_out, seq_lens, held_out, row_offsets, positions, slots, max_rows, counts, true, true};
     const int blocks = std::min(num_sms(), std::max(ceil_div(max_rows, 2 * PP_THREADS), ceil_div(batch, 128)));
     a.report = blocks <= 1 || !(seq_lens == ctx_lens || held_out == held || ring_at_out == ring_at);
-    int rc = launch_serve("paged_plan_kernel", paged_plan_kernel, dim3(std::max(blocks, 1)), dim3(PP_THREADS), 0, 1, false, a);
+    int rc = launch_serve("paged_plan_kernel", paged_plan_kernel, dim3(std::max(blocks, 1)), dim3(PP_THREADS), 0, 1, true, a);
     if (rc || a.report) return rc;
     a.expand = false;
     a.report = true;
-    return launch_serve("paged_plan_kernel", paged_plan_kernel, dim3(1), dim3(PP_THREADS), 0, 1, false, a);
+    return launch_serve("paged_plan_kernel", paged_plan_kernel, dim3(1), dim3(PP_THREADS), 0, 1, true, a);
 }

@@ -59,6 +59,7 @@ template <bool HALVES, int W>
 __global__ void __launch_bounds__(RS_THREADS) rope_scaled_kernel(const __grid_constant__ RopeArgs a) {
     constexpr int AT_ONCE = 4;
     __shared__ float2 s_cs[RS_MAX_PAIRS];
+    short_begin();
     const int64_t t = blockIdx.x;
     const int half = a.rot / 2;
     const int turned = HALVES ? half / W : a.rot / W;       // steps of a head that turn, the others copy
@@ -156,7 +157,8 @@ static int launch_rope(RopeArgs a, int64_t ntok) {
     const int steps = ceil_div((a.heads + a.kv) * a.items, RS_THREADS);
     // one token per block where that fills the device; fewer tokens: their heads are dealt out
     const int shares = ntok >= 2 * num_sms() ? 1 : std::min<int>(steps, ceil_div(2 * num_sms(), (int)ntok));
-    return launch_serve("rope_scaled_kernel", rope_scaled_kernel<HALVES, W>, dim3((unsigned)ntok, shares), dim3(RS_THREADS), 0, 1, false, a);
+    const dim3 grid((unsigned)ntok, shares);
+    return launch_serve("rope_scaled_kernel", rope_scaled_kernel<HALVES, W>, grid, dim3(RS_THREADS), 0, 1, short_grid(grid), a);
 }
 
 }  // namespace b200

@@ -2,7 +2,7 @@
 // at run time, launches with clusters and programmatic order.
 #pragma once
 
-#include "common.cuh"
+#include "stream.cuh"
 #include "../../include/b200serve.h"
 
 namespace b200 {
@@ -68,7 +68,9 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
 
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// cluster > 1: that many blocks along x form a cluster; early: the kernel may start while the one before it ends (it waits by itself).
+// cluster > 1: that many blocks along x form a cluster; early: the kernel is set up while the one before it ends (it waits by itself, in
+// its first statement: pdl_wait() or short_begin()).  Grids of short_grid() take it; larger ones would hold SMs that the kernel before
+// them still has use for.
 template <typename Kern, typename Args>
 static int launch_serve(const char* name, Kern kern, dim3 grid, dim3 block, size_t smem, int cluster, bool early, const Args& a) {
     cudaLaunchConfig_t cfg = {};

@@ -135,7 +135,8 @@ template <bool WIDE, bool GREEDY>
 __global__ void __launch_bounds__(VD_THREADS, VD_RESIDENT) verify_stats_kernel(const __grid_constant__ VerifyArgs a) {
     constexpr int HALF = 4 * VD_THREADS, EACH = 16, STEP = VD_THREADS * EACH;
     __shared__ VdPart s_part[VD_WARPS];
-    asm volatile("griddepcontrol.launch_dependents;");
+    pdl_launch_dependents();
+    pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int live = min(a.offsets[a.batch], a.rows), c0 = blockIdx.x * a.chunk, c1 = min(a.V, c0 + a.chunk);
     for (int row = blockIdx.y; row < live; row += gridDim.y) {
@@ -241,7 +242,7 @@ __global__ void __launch_bounds__(VD_THREADS, VD_RESIDENT) verify_pick_kernel(co
     const int rank = (int)cluster.block_rank(), b = blockIdx.x / VD_CLUSTER, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     vd_table(s_pow);
     __syncthreads();
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    pdl_wait();
     const int first = max(a.offsets[b], 0), count = min(a.offsets[b + 1], a.rows) - first, drafts = min(count - 1, a.max_drafts);
     int32_t* tokens = a.tokens + (int64_t)b * (a.max_drafts + 1);
     if (count <= 0) {                              // no rows: the whole cluster leaves
@@ -543,12 +544,12 @@ int b200_verify_drafts(const float* logits, int64_t logits_stride, const float* 
         const dim3 grid(a.chunks, std::min(rows, 65535));
         auto kern = wide ? (greedy ? verify_stats_kernel<true, true> : verify_stats_kernel<true, false>)
                          : (greedy ? verify_stats_kernel<false, true> : verify_stats_kernel<false, false>);
-        rc = launch_serve("verify_stats_kernel", kern, grid, block, 0, 1, false, a);
+        rc = launch_serve("verify_stats_kernel", kern, grid, block, 0, 1, short_grid(grid), a);
         if (rc) return rc;
     }
     auto kern = wide ? (greedy ? verify_pick_kernel<true, true> : verify_pick_kernel<true, false>)
                      : (greedy ? verify_pick_kernel<false, true> : verify_pick_kernel<false, false>);
-    return launch_serve("verify_pick_kernel", kern, dim3(batch * VD_CLUSTER), block, 0, VD_CLUSTER, rows > 0, a);
+    return launch_serve("verify_pick_kernel", kern, dim3(batch * VD_CLUSTER), block, 0, VD_CLUSTER, true, a);
 }
 
 }  // extern "C"
