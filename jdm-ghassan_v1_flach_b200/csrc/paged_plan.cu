@@ -54,6 +54,7 @@ __global__ void __launch_bounds__(PP_THREADS) paged_plan_kernel(const __grid_con
     const long long head = a.at[0], tail = a.at[1];
     const bool sound = head >= 0 && tail >= head && tail - head <= (long long)a.ring_size;
     const long long avail = sound ? tail - head : 0;
+    const uint32_t ring_head = sound ? (uint32_t)(head % a.ring_size) : 0, ring_tail = sound ? (uint32_t)(tail % a.ring_size) : 0;
     if (tid < 2) s_most[tid] = 0;
     if (tid == 2) s_refused = 0;
     int ctx[PP_EACH], fresh[PP_EACH], held[PP_EACH];
@@ -90,11 +91,14 @@ __global__ void __launch_bounds__(PP_THREADS) paged_plan_kernel(const __grid_con
         if (lane == 31) s_part[warp][k] = v;
     }
     __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 3; ++k)
-        for (int w = 0; w < warp; ++w) before[k] += s_part[w][k];
+    const int warps = (a.batch + 32 * PP_EACH - 1) / (32 * PP_EACH);        // that have requests
     long long all_back = 0;
-    for (int w = 0; w < PP_THREADS / 32; ++w) all_back += s_part[w][2];
+    for (int w = 0; w < warps; ++w) {
+        if (w < warp)
+#pragma unroll
+            for (int k = 0; k < 3; ++k) before[k] += s_part[w][k];
+        all_back += s_part[w][2];
+    }
     // admission; the largest sums among the admitted are the step's totals
     bool ok[PP_EACH];
     int refused = 0, most_rows = 0, most_take = 0;
@@ -163,7 +167,6 @@ __global__ void __launch_bounds__(PP_THREADS) paged_plan_kernel(const __grid_con
         }
     }
     if (!a.expand) return;
-    const uint32_t ring_head = sound ? (uint32_t)(head % a.ring_size) : 0, ring_tail = sound ? (uint32_t)(tail % a.ring_size) : 0;
     auto ring_index = [&](uint32_t from, uint32_t j) {      // both below the ring's size
         const uint32_t i = from + j;
         return i >= a.ring_size ? i - a.ring_size : i;
