@@ -26,6 +26,7 @@
 // same keys: idle ones where the pairs are no multiple, 149 us on the drafts below.)  Keys come through a ring of each warp's own in
 // shared memory that cp.async fills one or two tiles ahead.
 #include <algorithm>
+#include <type_traits>
 
 #include "serve.cuh"
 
@@ -36,9 +37,9 @@ constexpr int A4_THREADS = A4_WARPS * 32;
 constexpr int A4_KEYS = 32;                      // keys of a warp's step
 constexpr int A4_ITEM = 3;                       // what an item's set-up costs, in units
 constexpr int A4_LEAST = 4;                      // units of a worker at the least
-constexpr int A4_RESIDENT = 3;                   // blocks on an SM: 168 registers a thread
-// Stages of a warp's ring, by its tiles of four pairs: two tiles take long enough to hide a load behind one.
-__host__ __device__ constexpr int a4_stages(int nt) { return nt == 1 ? 3 : 2; }
+constexpr int A4_STAGES = 2;
+// Blocks on an SM, by a warp's tiles of four pairs: 168 registers a thread, or 255.
+__host__ __device__ constexpr int a4_resident(int nt) { return nt > 2 ? 2 : 3; }
 // A warp's query fragments where they stay in shared memory: 32 registers that two tiles of pairs have more use for.
 __host__ __device__ constexpr int a4_query_bytes(int hd, int nt) { return nt > 1 ? nt * (hd / 32) * 32 * 16 : 0; }
 
@@ -177,9 +178,9 @@ __device__ __forceinline__ A4Range a4_range(const Kv4AttnArgs& a, const A4Seq& s
 }
 
 template <int HD, int KIND, int NT>
-__global__ void __launch_bounds__(A4_THREADS, A4_RESIDENT) attn_kv4_kernel(const __grid_constant__ Kv4AttnArgs a) {
+__global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(const __grid_constant__ Kv4AttnArgs a) {
     using ST = A4Stage<HD, KIND>;
-    constexpr int NB = ST::NB, PAIRS = 4 * NT, STAGES = a4_stages(NT), RING = STAGES * ST::BYTES;
+    constexpr int NB = ST::NB, PAIRS = 4 * NT, STAGES = A4_STAGES, RING = STAGES * ST::BYTES;
     constexpr uint32_t LOW = 0x000F000Fu, UP = 0x00F000F0u;      // code * 2^-24, code * 2^-20
     constexpr uint32_t LESS_8 = 0x80088008u, LESS_8_UP = 0x80808080u;        // -8 of each
     constexpr float ROUND = 12582912.0f;                         // 1.5 * 2^23
@@ -696,19 +697,21 @@ __global__ void __launch_bounds__(THREADS) attn_kv4_join_kernel(const __grid_con
 template <int HD>
 static int launch_a4_join(const Kv4AttnArgs& a, int items) {
     constexpr int THREADS = 2 * HD, AT_ONCE = HD / 16;
+    if (a.pairs > 8)
+        return launch_serve("attn_kv4_join_kernel", attn_kv4_join_kernel<HD, 4 * HD, 4>, dim3(a.workers), dim3(4 * HD), 0, 1, true, a);
     if (items > num_sms()) return launch_serve("attn_kv4_join_kernel", attn_kv4_join_kernel<HD, THREADS, AT_ONCE>, dim3(a.workers), dim3(THREADS), 0, 1, true, a);
     return launch_serve("attn_kv4_join_kernel", attn_kv4_join_kernel<HD, 512, 8>, dim3(num_sms()), dim3(512), 0, 1, true, a);
 }
 
 // Tiles of four pairs that a warp takes at once, from the most pairs that a sequence has for a KV head.
-static int a4_tiles(int64_t most) { return most <= 4 ? 1 : 2; }
-static int a4_blocks() { return A4_RESIDENT * num_sms(); }
+static int a4_tiles(int64_t most) { return most <= 4 ? 1 : most <= 32 ? 2 : 4; }
+static int a4_blocks(int nt) { return a4_resident(nt) * num_sms(); }
 
 template <int HD, int KIND, int NT>
 static int launch_a4(const Kv4AttnArgs& a, int blocks) {
     auto kern = attn_kv4_kernel<HD, KIND, NT>;
-    constexpr int smem = A4_WARPS * (a4_stages(NT) * A4Stage<HD, KIND>::BYTES + a4_query_bytes(HD, NT));
-    if (smem > 48 * 1024) B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    constexpr int smem = A4_WARPS * (A4_STAGES * A4Stage<HD, KIND>::BYTES + a4_query_bytes(HD, NT));
+    if (smem + 2048 > 48 * 1024) B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     return launch_serve("attn_kv4_kernel", kern, dim3(blocks), dim3(A4_THREADS), smem, 1, true, a);
 }
 
@@ -724,7 +727,7 @@ int b200_attention_paged_kv4_workspace(int H, int KV, int hd, int max_rows, size
     B200_REQUIRE(bytes, "attention_paged_kv4_workspace: null pointer");
     B200_REQUIRE(H >= 1 && H % KV == 0 && max_rows >= 1, "attention_paged_kv4_workspace: H must be a positive multiple of KV, max_rows positive");
     const int nt = a4_tiles((int64_t)max_rows * (H / KV));
-    *bytes = (size_t)a4_blocks() * A4_WARPS * (sizeof(A4Item) + (size_t)2 * 4 * nt * (hd + 4) * sizeof(float));
+    *bytes = (size_t)a4_blocks(nt) * A4_WARPS * (sizeof(A4Item) + (size_t)2 * 4 * nt * (hd + 4) * sizeof(float));
     return B200_OK;
 }
 
@@ -746,16 +749,16 @@ int b200_attention_paged_kv4(const float* q, int64_t q_stride, const int32_t* ro
     rc = b200_attention_paged_kv4_workspace(H, KV, hd, max_rows, &need);
     if (rc) return rc;
     B200_REQUIRE(workspace_bytes >= need, "%s: the workspace has %zu bytes of %zu", who, workspace_bytes, need);
-    const int nt = a4_tiles((int64_t)max_rows * (H / KV)), blocks = a4_blocks(), workers = blocks * A4_WARPS;
+    const int nt = a4_tiles((int64_t)max_rows * (H / KV)), blocks = a4_blocks(nt), workers = blocks * A4_WARPS;
     Kv4AttnArgs a{q, q_stride, row_offsets, static_cast<const uint8_t*>(pages), num_pages, page_table, seq_lens, out, out_stride, batch,
                   max_pages, page, H, KV, H / KV, FastDiv(page), FastDiv(H / KV), FastDiv(4 * nt), Kv4Page(page, KV, hd, kind), scale, window, 4 * nt, workers,
                   reinterpret_cast<float*>(static_cast<A4Item*>(workspace) + workers), static_cast<A4Item*>(workspace)};
-    if (hd == 64)
-        rc = kind == 1 ? (nt == 1 ? launch_a4<64, 1, 1>(a, blocks) : launch_a4<64, 1, 2>(a, blocks))
-                       : (nt == 1 ? launch_a4<64, 0, 1>(a, blocks) : launch_a4<64, 0, 2>(a, blocks));
-    else
-        rc = kind == 1 ? (nt == 1 ? launch_a4<128, 1, 1>(a, blocks) : launch_a4<128, 1, 2>(a, blocks))
-                       : (nt == 1 ? launch_a4<128, 0, 1>(a, blocks) : launch_a4<128, 0, 2>(a, blocks));
+    auto go = [&](auto tiles) {
+        constexpr int NT = decltype(tiles)::value;
+        return hd == 64 ? (kind == 1 ? launch_a4<64, 1, NT>(a, blocks) : launch_a4<64, 0, NT>(a, blocks))
+                        : (kind == 1 ? launch_a4<128, 1, NT>(a, blocks) : launch_a4<128, 0, NT>(a, blocks));
+    };
+    rc = nt == 1 ? go(std::integral_constant<int, 1>()) : nt == 2 ? go(std::integral_constant<int, 2>()) : go(std::integral_constant<int, 4>());
     if (rc) return rc;
     const int64_t items = (int64_t)batch * KV * (((int64_t)max_rows * (H / KV) + a.pairs - 1) / a.pairs);       // at the most
     return hd == 64 ? launch_a4_join<64>(a, (int)std::min<int64_t>(items, 1 << 30)) : launch_a4_join<128>(a, (int)std::min<int64_t>(items, 1 << 30));
