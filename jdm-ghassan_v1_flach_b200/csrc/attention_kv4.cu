@@ -36,7 +36,7 @@ constexpr int A4_WARPS = 4;
 constexpr int A4_THREADS = A4_WARPS * 32;
 constexpr int A4_KEYS = 32;                      // keys of a warp's step
 constexpr int A4_ITEM = 3;                       // what an item's set-up costs, in units
-constexpr int A4_LEAST = 4;                      // units of a worker at the least
+constexpr int A4_LEAST = 2;                      // units of a worker at the least (one sequence of 300 tokens: 9.2 us, of 4: 10.9; 1 and 4097 tokens: more pieces than it saves)
 constexpr int A4_STAGES = 2;
 // Blocks on an SM, by a warp's tiles of four pairs: 168 registers a thread, or 255.
 __host__ __device__ constexpr int a4_resident(int nt) { return nt > 2 ? 2 : 3; }
@@ -703,8 +703,10 @@ static int launch_a4_join(const Kv4AttnArgs& a, int items) {
     return launch_serve("attn_kv4_join_kernel", attn_kv4_join_kernel<HD, 512, 8>, dim3(num_sms()), dim3(512), 0, 1, true, a);
 }
 
-// Tiles of four pairs that a warp takes at once, from the most pairs that a sequence has for a KV head.
-static int a4_tiles(int64_t most) { return most <= 4 ? 1 : most <= 32 ? 2 : 4; }
+// Tiles of four pairs that a warp takes at once, from the most pairs that a sequence has for a KV head.  A tile's keys are unpacked
+// once for all of its pairs, but pairs that are not there cost as much as others: 16 sequences, 5 rows of 32/8 heads (20 pairs)
+// 69 us in eights, 84 in sixteens; 72 pairs of 12/4 heads 93 and 101; 96 pairs 223 and 212; prompts' pieces of 300 to 900 pairs 84 and 79.
+static int a4_tiles(int64_t most) { return most <= 4 ? 1 : most <= 128 ? 2 : 4; }
 static int a4_blocks(int nt) { return a4_resident(nt) * num_sms(); }
 
 template <int HD, int KIND, int NT>
@@ -740,6 +742,8 @@ int b200_attention_paged_kv4(const float* q, int64_t q_stride, const int32_t* ro
     int rc = kv4_check(who, num_pages, page, KV, hd, kind);
     if (rc) return rc;
     B200_REQUIRE(H >= 1 && H % KV == 0, "%s: H must be a positive multiple of KV", who);
+    B200_REQUIRE(batch <= 1 << 24, "%s: too many sequences", who);
+    if (window >= (int64_t)max_pages * page) window = 0;         // wider than any sequence
     B200_REQUIRE(max_rows >= 1 && max_pages >= 1 && (int64_t)max_pages * page <= 0x7fffff00, "%s: bad max_rows or max_pages", who);
     B200_REQUIRE(q && pages && page_table && seq_lens && out && workspace, "%s: null pointer", who);
     B200_REQUIRE(aligned16(q) && aligned16(out) && aligned16(pages) && aligned16(workspace) && q_stride % 4 == 0 && out_stride % 4 == 0,

@@ -325,20 +325,11 @@ __global__ void __launch_bounds__(VD_THREADS, VD_RESIDENT) verify_pick_kernel(co
         auto masses = [&](int at, const Four& f, bool from_p, double (&r)[4]) {
             float hi[4], lo[4];
             weights(f, hi, lo);
+            const float y[4] = {f.q.x, f.q.y, f.q.z, f.q.w};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) r[k] = (double)hi[k] + (double)lo[k];
-            if (from_p) return;
-            if (q) {
-                const float y[4] = {f.q.x, f.q.y, f.q.z, f.q.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    r[k] = fma(-(double)y[k], z, r[k]);
-                    if (!(r[k] > 0.0)) r[k] = 0.0;
-                }
-            } else if ((unsigned)(without - at) < 4u) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (at + k == without) r[k] = 0.0;
+            for (int k = 0; k < 4; ++k) {
+                r[k] = !from_p && q ? fma(-(double)y[k], z, (double)hi[k]) : (double)hi[k];
+                r[k] = r[k] > 0.0 && (from_p || at + k != without) ? fmax(r[k] + (double)lo[k], 0.0) : 0.0;
             }
         };
         const int own = (rank * VD_WARPS + warp) * seg;
@@ -423,7 +414,7 @@ __global__ void __launch_bounds__(VD_THREADS, VD_RESIDENT) verify_pick_kernel(co
         const float u = a.uniforms[first + count - 1];
         const double mark = (u > 0.0f ? fmin((double)u, 1.0 - 1.0 / 16777216.0) : 0.0) * total;
         const unsigned even = __ballot_sync(0xffffffffu, lane_from <= mark && mark < lane_mid), odd = __ballot_sync(0xffffffffu, lane_mid <= mark && mark < lane_to);
-        const int holder = even ? __ffs(even) - 1 : __ffs(odd) - 1;                  // lane whose segments hold the draw: there is one
+        const int holder = max(0, even ? __ffs(even) - 1 : __ffs(odd) - 1);          // lane whose segments hold the draw: there is one
         const int which = 2 * holder + (even == 0);
         if (which / VD_WARPS == rank) {            // this block walks the segment again, its warps a step each
             double run = __shfl_sync(0xffffffffu, even ? lane_from : lane_mid, holder);
@@ -453,7 +444,7 @@ __global__ void __launch_bounds__(VD_THREADS, VD_RESIDENT) verify_pick_kernel(co
                 __syncthreads();
             }
             if (warp == 0) {
-                const int at = from + found * 128 + 4 * lane;
+                const int at = from + max(found, 0) * 128 + 4 * lane;
                 double r[4];
                 masses(at, load(at, !from_p && q), from_p, r);
                 const double sum = (r[0] + r[1]) + (r[2] + r[3]);
@@ -476,7 +467,7 @@ __global__ void __launch_bounds__(VD_THREADS, VD_RESIDENT) verify_pick_kernel(co
                 hit = __reduce_min_sync(0xffffffffu, hit);
                 last = __reduce_max_sync(0xffffffffu, last);
                 // sums in another order may end a rounding short of the mark: the last one that has mass
-                if (lane == 0) tokens[n] = hit != 0x7fffffff ? hit : last;
+                if (lane == 0) tokens[n] = hit != 0x7fffffff ? hit : last >= 0 ? last : min(from, a.V - 1);
             }
         }
         cluster.sync();                            // nobody leaves while its masses are read

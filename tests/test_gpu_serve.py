@@ -400,6 +400,35 @@ def test_attention_far_into_a_large_pool():
     assert np.array_equal(host(b), so.values(*so.quantize(-x, 1), 1).astype(np.float32))
 
 
+def test_attention_with_a_window_beyond_every_length():
+    r = np.random.default_rng(59)
+    lens, rows = [70, 5], [3, 9]                               # more rows than tokens, too
+    cache, table, kv = make_cache(r, lens, 16, 2, 64, 1)
+    q, offs = dev(r.standard_normal((12, 4, 64)).astype(np.float32)), i32([0, 3, 12])
+    got = []
+    for window in (0, 2 ** 31 - 1, 96, -5):
+        out = empty((12, 4, 64))
+        call_attention(q, 256, offs, dev(cache.bytes), cache.num_pages, i32(table), i32(lens), out, 256, 9, 16, 4, 2, 64, 1, 0.125, window)
+        got.append(out)
+    assert all(torch.equal(got[0], o) for o in got[1:]) and (got[0][3:7] == 0).all()
+
+
+def test_attention_of_many_sequences():
+    """More sequences than a block has threads, many of them without rows or tokens."""
+    r = np.random.default_rng(61)
+    B, H, KV, hd, page = 700, 4, 2, 64, 16
+    lens = [int(x) for x in r.integers(0, 90, B)]
+    rows = [int(x) for x in r.choice([0, 0, 1, 2], B)]
+    rows[-3:] = [0, 0, 0]
+    cache, table, kv = make_cache(r, lens, page, KV, hd, 0)
+    offs = np.concatenate([[0], np.cumsum(rows)])
+    q = r.standard_normal((int(offs[-1]), H, hd)).astype(np.float32)
+    out = empty(q.shape)
+    call_attention(dev(q), H * hd, i32(offs), dev(cache.bytes), cache.num_pages, i32(table), i32(lens), out, H * hd, 2, page, H, KV, hd, 0, 0.125, 0)
+    want = np.concatenate([so.attention(q, offs[b], rows[b], lens[b], *kv[b], 0.125, 0) for b in range(B)])
+    assert np.abs(host(out) - want).max() <= attention_bound(q, kv, 0.125)
+
+
 def test_attention_is_the_same_every_time():
     """Whatever the workspace held, and whatever else is in the batch's order of blocks: the same bits twice."""
     r = np.random.default_rng(56)
@@ -580,6 +609,33 @@ def test_verify_falls_back_where_the_rest_has_no_mass():
     q = np.full((2, V), 1 / V, np.float32)
     acc, tok = run_verify(logits, q, [0, 5], [0, 2], 1.0, [1.0, 0.5], 1)
     assert acc[0] == 0 and tok[0].tolist() == [32, -1]
+
+
+def test_verify_where_p_and_q_nearly_agree():
+    """What is left of p - q is rounding on most of the vocabulary and a little on a few tokens, all in one segment of a warp."""
+    r = np.random.default_rng(12)
+    V, n = 20000, 16
+    logits = r.standard_normal((2 * n, V)).astype(np.float32)
+    p = np.exp(logits.astype(np.float64))
+    p /= p.sum(1, keepdims=True)
+    q = p.copy()
+    q[:, 7000:7004] *= 0.5                             # the rest's mass: half of these
+    q[:, 3] += (p - q).sum(1)
+    ids = np.tile([0, 3], n)
+    u = np.tile([1 - 2.0 ** -24, 0.0], n)
+    u[1::2] = (np.arange(n) + 0.5) / n
+    got = run_verify(logits, q.astype(np.float32), ids, np.arange(0, 2 * n + 1, 2), 1.0, u, 1)
+    assert (got[0] == 0).all()
+    # of 4 tokens' mass; what q's rounding to fp32 leaves elsewhere is 2^-25 of p, together 2^-26 of 1 at most
+    for b in range(n):
+        part = (p - q)[2 * b, 7000:7004]
+        slack = 2.0 ** -24 / part.sum()
+        x = got[1][b, 0]
+        if 7000 <= x < 7004:
+            c = np.cumsum(part) / part.sum()
+            assert c[x - 7000] - part[x - 7000] / part.sum() - slack <= u[2 * b + 1] <= c[x - 7000] + slack
+        else:
+            assert slack > 0.01 and 0 <= x < V
 
 
 def test_verify_greedy_ties_go_to_the_lowest():

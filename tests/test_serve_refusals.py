@@ -74,7 +74,7 @@ ATTN = dict(q=P, qs=1024, offsets=P, pages=P, num_pages=10, table=P, lens=P, out
 @pytest.mark.parametrize("change", [dict(hd=96), dict(kind=3), dict(H=7), dict(H=0), dict(KV=0), dict(rows=0), dict(max_pages=0), dict(page=0),
                                     dict(q=None), dict(out=None), dict(pages=None), dict(table=None), dict(lens=None), dict(work=None),
                                     dict(q=P + 4), dict(out=P + 8), dict(pages=P + 4), dict(work=P + 8), dict(qs=1022), dict(qs=1025), dict(os=1020),
-                                    dict(size=0), dict(num_pages=1 << 28), dict(max_pages=1 << 28)])
+                                    dict(size=0), dict(batch=(1 << 24) + 1), dict(num_pages=1 << 28), dict(max_pages=1 << 28)])
 def test_attention(change):
     refused("b200_attention_paged_kv4", ATTN, **change)
 
@@ -84,7 +84,7 @@ VERIFY = dict(logits=P, ls=100, draft=P, ds=100, ids=P, offsets=P, batch=2, rows
 
 @pytest.mark.parametrize("change", [dict(logits=None), dict(ids=None), dict(offsets=None), dict(u=None), dict(accepted=None), dict(tokens=None),
                                     dict(work=None), dict(work=P + 8), dict(size=8), dict(V=0), dict(rows=-1), dict(ls=99), dict(ds=99), dict(k=-1),
-                                    dict(k=256), dict(T=float("nan")), dict(T=float("inf")), dict(T=1e-42)])
+                                    dict(k=256), dict(T=float("nan")), dict(T=float("inf")), dict(T=2e30), dict(T=1e-42)])
 def test_verify(change):
     refused("b200_verify_drafts", VERIFY, **change)
 
