@@ -625,40 +625,53 @@ __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(c
 }
 
 // Items that a worker began and others went on with, a block each: a thread per four dims of a pair and group of pieces, AT_ONCE pieces at
-// a time.  Many items have few pieces: a block with a thread per column or two.  Few items, that is few sequences, have many.
+// a time.  Many items have few pieces: a block with a thread per column or two for every worker, which reads the pieces that there would
+// be at the same time as how many there are.  Few items, that is few sequences, have many: large blocks for several workers each.
 template <int HD, int THREADS, int AT_ONCE>
-__global__ void __launch_bounds__(THREADS) attn_kv4_join_kernel(const __grid_constant__ Kv4AttnArgs a) {
+__global__ void __launch_bounds__(THREADS, 4096 / AT_ONCE / THREADS) attn_kv4_join_kernel(const __grid_constant__ Kv4AttnArgs a) {
     __shared__ float4 s_o[THREADS];
     __shared__ float2 s_ml[THREADS];
     const int columns = a.pairs * (HD / 4), groups = THREADS / columns, lane = threadIdx.x & 31;
+    const int group = threadIdx.x / columns, col = threadIdx.x % columns, p = col / (HD / 4), c = col % (HD / 4) * 4;
     pdl_wait();
-    const int mine = blockIdx.x + lane * gridDim.x;              // the workers of this block
-    unsigned left = __ballot_sync(0xffffffffu, mine < a.workers && __ldcg(&a.item[min(mine, a.workers - 1)].more) > 0);
+    unsigned left = 1;                                           // bit k: worker blockIdx.x + k gridDim.x began something
+    if (gridDim.x < (unsigned)a.workers) {
+        const int mine = blockIdx.x + lane * gridDim.x;
+        left = __ballot_sync(0xffffffffu, mine < a.workers && __ldcg(&a.item[min(mine, a.workers - 1)].more) > 0);
+    }
     for (; left; left &= left - 1) {
         const int worker = blockIdx.x + (__ffs(left) - 1) * gridDim.x;
-        const A4Item it = a.item[worker];
-        const int group = threadIdx.x / columns, col = threadIdx.x % columns, p = col / (HD / 4), c = col % (HD / 4) * 4;
         // piece i: the worker's own second slot, then the first slots of those behind it
         const float* pieces = a.piece + ((int64_t)(2 * worker) * a.pairs + p) * (HD + 4);
-        float mm = -INFINITY, ll = 0.0f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i0 = group; i0 <= it.more; i0 += AT_ONCE * groups) {
-            float2 ml[AT_ONCE];
-            float4 v[AT_ONCE];
+        float2 ml[AT_ONCE];
+        float4 v[AT_ONCE];
+        auto load = [&](int i0, int most) {
 #pragma unroll
             for (int k = 0; k < AT_ONCE; ++k) {
                 const int i = i0 + k * groups;
-                ml[k] = make_float2(-INFINITY, 0.0f);
-                v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (i <= it.more) {
+                if (i <= most) {
                     const float* s = pieces + (int64_t)(2 * i + (i == 0)) * a.pairs * (HD + 4);
                     ml[k] = __ldcg(reinterpret_cast<const float2*>(s + HD));
                     v[k] = __ldcg(reinterpret_cast<const float4*>(s + c));
                 }
             }
+        };
+        load(group, a.workers - 1 - worker);
+        const A4Item it = a.item[worker];
+        if (it.more == 0) continue;
+        float mm = -INFINITY, ll = 0.0f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i0 = group; i0 <= it.more; i0 += AT_ONCE * groups) {
+            if (i0 != group) load(i0, it.more);
             float top = mm;
 #pragma unroll
-            for (int k = 0; k < AT_ONCE; ++k) top = fmaxf(top, ml[k].x);
+            for (int k = 0; k < AT_ONCE; ++k) {
+                if (i0 + k * groups > it.more) {                 // not there, whatever was read
+                    ml[k] = make_float2(-INFINITY, 0.0f);
+                    v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+                top = fmaxf(top, ml[k].x);
+            }
             const float base = top == -INFINITY ? 0.0f : top, old = a4_exp2(mm - base);
             ll *= old;
             acc.x *= old; acc.y *= old; acc.z *= old; acc.w *= old;
@@ -671,17 +684,17 @@ __global__ void __launch_bounds__(THREADS) attn_kv4_join_kernel(const __grid_con
             mm = top;
         }
         if (groups > 1) {
-            __syncthreads();                                 // the item before is read
+            __syncthreads();                                     // the item before is read
             s_o[threadIdx.x] = acc;
             s_ml[threadIdx.x] = make_float2(mm, ll);
             __syncthreads();
             if (group == 0)
                 for (int i = 1; i < groups; ++i) {
-                    const float2 ml = s_ml[i * columns + threadIdx.x];
-                    const float4 v = s_o[i * columns + threadIdx.x];
-                    const float top = fmaxf(mm, ml.x), base = top == -INFINITY ? 0.0f : top, f0 = a4_exp2(mm - base), f1 = a4_exp2(ml.x - base);
-                    ll = ll * f0 + ml.y * f1;
-                    acc.x = acc.x * f0 + v.x * f1; acc.y = acc.y * f0 + v.y * f1; acc.z = acc.z * f0 + v.z * f1; acc.w = acc.w * f0 + v.w * f1;
+                    const float2 other = s_ml[i * columns + threadIdx.x];
+                    const float4 w = s_o[i * columns + threadIdx.x];
+                    const float top = fmaxf(mm, other.x), base = top == -INFINITY ? 0.0f : top, f0 = a4_exp2(mm - base), f1 = a4_exp2(other.x - base);
+                    ll = ll * f0 + other.y * f1;
+                    acc.x = acc.x * f0 + w.x * f1; acc.y = acc.y * f0 + w.y * f1; acc.z = acc.z * f0 + w.z * f1; acc.w = acc.w * f0 + w.w * f1;
                     mm = top;
                 }
         }
@@ -696,7 +709,7 @@ __global__ void __launch_bounds__(THREADS) attn_kv4_join_kernel(const __grid_con
 
 template <int HD>
 static int launch_a4_join(const Kv4AttnArgs& a, int items) {
-    constexpr int THREADS = 2 * HD, AT_ONCE = HD / 16;
+    constexpr int THREADS = 2 * HD, AT_ONCE = 4;
     if (a.pairs > 8)
         return launch_serve("attn_kv4_join_kernel", attn_kv4_join_kernel<HD, 4 * HD, 4>, dim3(a.workers), dim3(4 * HD), 0, 1, true, a);
     if (items > num_sms()) return launch_serve("attn_kv4_join_kernel", attn_kv4_join_kernel<HD, THREADS, AT_ONCE>, dim3(a.workers), dim3(THREADS), 0, 1, true, a);
