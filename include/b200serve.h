@@ -24,7 +24,7 @@
  * d * code + m.  kind 0 holds the codes and scales of b200_quantize, bit for bit; kind 1 as well, but that its step is
  * (max - min) * fp32(1/15), not a division: its last bit may differ and with it the code of a value on the border of two.  d and m beyond
  * the range of fp16 are kept as +-65504 (every stored value is finite).  Slot s is token s % page of page s / page;
- * num_pages * page must fit in 31 bits. */
+ * num_pages * page must fit in 31 bits, KV * page be at most 2^23. */
 #ifndef B200SERVE_H
 #define B200SERVE_H
 

@@ -55,7 +55,7 @@ struct Kv4AttnArgs {
     int64_t os;
     int batch, max_pages, page, H, KV, group;
     FastDiv by_page, by_group, by_pairs;
-    Kv4Page part;
+    uint32_t page_bytes, k_scale, v_code;        // of a page, and of its parts
     float scale;
     int window;
     int pairs, workers;                          // pairs of a tile; warps of the grid
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(c
         seq = a4_seq(a, ++b);
     }
 
-    const bool wide = a.page % A4_KEYS == 0;                     // a warp's keys lie in one page
+    const bool halves = a.page % 16 == 0;                        // sixteen keys lie in one page
     constexpr int step = A4_KEYS;
     constexpr bool Q_SHARED = NT > 1;
     uint8_t* ring = a4_ring + warp * RING;
@@ -257,13 +257,16 @@ __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(c
         const uint32_t kdst = ring_at + ((lkey & 8) + 2 * (lkey & 3) + ((lkey >> 2) & 1)) * ST::ROW + lpiece;
         const uint32_t vdst = ring_at + ST::V + lkey * ST::ROW + (HD == 128 ? lpiece ^ ((lkey & 2) * 16) : lpiece);
         const uint32_t sdst = ring_at + ST::KS + lane * ST::SROW;
+        const int kv_row = kv * a.page;
+        // Page and token in it of the tile's keys: a lane has the first key of its half (sixteen keys lie in one page), or, where pages do
+        // not allow that, its own key.
         struct Place {
-            int id, off;                                         // page and token in it: of the tile's first key, or (not wide) of the lane's
+            int id, off;
         };
         auto place = [&](int k) {
             Place pl{-1, 0};
             if (k < kend) {
-                const int key = wide ? k : min(k + lane, kend - 1), p = (int)a.by_page.div(key);
+                const int key = min(k + (halves ? lane & 16 : lane), kend - 1), p = (int)a.by_page.div(key);
                 pl.id = table[p];
                 pl.off = key - p * a.page;
             }
@@ -272,39 +275,37 @@ __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(c
         auto issue = [&](int s, int k, Place pl) {
             const uint32_t so = s * ST::BYTES;
             const bool there = (uint32_t)pl.id < (uint32_t)a.num_pages;
-            const uint8_t* at = a.pages + (int64_t)(there ? pl.id : 0) * a.part.bytes;
-            const int64_t row = (int64_t)kv * a.page + pl.off;
-            if (wide && there && k + A4_KEYS <= kend) {
-                const uint8_t* p = at + row * ST::ROW + lkey * ST::ROW + lpiece;
-                const uint8_t* ps = at + a.part.k_scale + (row + lane) * ST::SROW;
-                const int64_t v_code = a.part.v_code;
+            const uint8_t* at = a.pages + (uint64_t)(there ? (uint32_t)pl.id : 0u) * a.page_bytes;
+            const uint8_t* codes = at + (uint32_t)(kv_row + pl.off) * ST::ROW;
+            const uint8_t* scales = at + a.k_scale + (uint32_t)(kv_row + pl.off + (halves ? lane & 15 : 0)) * ST::SROW;
+            if (halves && k + A4_KEYS <= kend && __all_sync(0xffffffffu, there)) {
+                const uint8_t* half[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    half[h] = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(codes), 16 * h)) + (lkey * ST::ROW + lpiece);
 #pragma unroll
                 for (int i = 0; i < A4_KEYS / PER; ++i) {
-                    a4_copy<16>(kdst + so + i * PER * ST::ROW, p + i * PER * ST::ROW);
-                    a4_copy<16>(vdst + so + i * PER * ST::ROW, p + v_code + i * PER * ST::ROW);
+                    const uint8_t* p = half[i * PER / 16] + i * PER % 16 * ST::ROW;
+                    a4_copy<16>(kdst + so + i * PER * ST::ROW, p);
+                    a4_copy<16>(vdst + so + i * PER * ST::ROW, p + a.v_code);
                 }
-                a4_copy<ST::SROW>(sdst + so, ps);
-                a4_copy<ST::SROW>(sdst + so + (ST::VS - ST::KS), ps + v_code);     // the V parts follow the K parts in the same order
+                a4_copy<ST::SROW>(sdst + so, scales);
+                a4_copy<ST::SROW>(sdst + so + (ST::VS - ST::KS), scales + a.v_code);       // the V parts follow the K parts in the same order
                 return;
             }
 #pragma unroll
             for (int i = 0; i < A4_KEYS / PER; ++i) {
-                const int key_of = i * PER + lkey;
-                const uint8_t* p = at + (row + (wide ? key_of : 0)) * ST::ROW;
-                bool ok = there;
-                if (!wide) {
-                    p = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(p), key_of));
-                    ok = __shfl_sync(0xffffffffu, there, key_of);
-                }
-                ok = ok && k + key_of < kend;
-                p = ok ? p + lpiece : a.pages;
+                const int key_of = i * PER + lkey, of = halves ? key_of & 16 : key_of;
+                const uint8_t* p = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(codes), of));
+                const bool ok = __shfl_sync(0xffffffffu, there, of) && k + key_of < kend;
+                p = ok ? p + (halves ? key_of & 15 : 0) * ST::ROW + lpiece : a.pages;
                 a4_copy<16>(kdst + so + i * PER * ST::ROW, p, ok);
-                a4_copy<16>(vdst + so + i * PER * ST::ROW, p + a.part.v_code, ok);
+                a4_copy<16>(vdst + so + i * PER * ST::ROW, p + a.v_code, ok);
             }
             const bool ok = k + lane < kend && there;
-            const uint8_t* p = ok ? at + (row + (wide ? lane : 0)) * ST::SROW : a.pages;
-            a4_copy<ST::SROW>(sdst + so, p + a.part.k_scale, ok);
-            a4_copy<ST::SROW>(sdst + so + (ST::VS - ST::KS), p + a.part.v_scale, ok);
+            const uint8_t* p = ok ? scales : a.pages;
+            a4_copy<ST::SROW>(sdst + so, p, ok);
+            a4_copy<ST::SROW>(sdst + so + (ST::VS - ST::KS), p + a.v_code, ok);
         };
         auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
 
@@ -767,8 +768,9 @@ int b200_attention_paged_kv4(const float* q, int64_t q_stride, const int32_t* ro
     if (rc) return rc;
     B200_REQUIRE(workspace_bytes >= need, "%s: the workspace has %zu bytes of %zu", who, workspace_bytes, need);
     const int nt = a4_tiles((int64_t)max_rows * (H / KV)), blocks = a4_blocks(nt), workers = blocks * A4_WARPS;
+    const Kv4Page part(page, KV, hd, kind);
     Kv4AttnArgs a{q, q_stride, row_offsets, static_cast<const uint8_t*>(pages), num_pages, page_table, seq_lens, out, out_stride, batch,
-                  max_pages, page, H, KV, H / KV, FastDiv(page), FastDiv(H / KV), FastDiv(4 * nt), Kv4Page(page, KV, hd, kind), scale, window, 4 * nt, workers,
+                  max_pages, page, H, KV, H / KV, FastDiv(page), FastDiv(H / KV), FastDiv(4 * nt), (uint32_t)part.bytes, (uint32_t)part.k_scale, (uint32_t)part.v_code, scale, window, 4 * nt, workers,
                   reinterpret_cast<float*>(static_cast<A4Item*>(workspace) + workers), static_cast<A4Item*>(workspace)};
     auto go = [&](auto tiles) {
         constexpr int NT = decltype(tiles)::value;

@@ -34,6 +34,7 @@ int kv4_check(const char* who, int num_pages, int page, int KV, int hd, int kind
     B200_REQUIRE(kind == 0 || kind == 1, "%s: kind must be 0 (Q4_0) or 1 (Q4_1)", who);
     B200_REQUIRE(KV >= 1 && KV <= 65536 && page >= 1 && num_pages >= 1, "%s: bad cache geometry", who);
     B200_REQUIRE((int64_t)num_pages * page <= 0x7fffffff, "%s: num_pages * page must fit in 31 bits", who);
+    B200_REQUIRE((int64_t)KV * page <= 1 << 23, "%s: a page may have %d rows (tokens times heads)", who, 1 << 23);      // under 2^31 bytes
     return B200_OK;
 }
 

@@ -54,7 +54,7 @@ def test_rope(change):
 STORE = dict(k=P, v=P, ks=256, vs=256, slots=P, n=3, pages=P, num_pages=10, page=16, KV=2, hd=128, kind=1)
 FETCH = dict(pages=P, num_pages=10, page=16, slots=P, n=3, k=P, v=P, ks=256, vs=256, KV=2, hd=128, kind=1)
 CACHE = [dict(hd=96), dict(hd=32), dict(hd=256), dict(kind=2), dict(kind=-1), dict(KV=0), dict(page=0), dict(num_pages=0), dict(pages=None),
-         dict(pages=P + 8), dict(slots=None), dict(ks=255), dict(vs=255), dict(num_pages=1 << 20, page=1 << 12)]
+         dict(pages=P + 8), dict(slots=None), dict(ks=255), dict(vs=255), dict(num_pages=1 << 20, page=1 << 12), dict(num_pages=1, page=(1 << 22) + 1)]
 
 
 @pytest.mark.parametrize("change", CACHE + [dict(k=None), dict(v=None)])
