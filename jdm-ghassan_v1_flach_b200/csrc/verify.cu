@@ -11,7 +11,7 @@
 // random, one draw in 10 000 (counted on rows of variance 6).  So the second kernel makes its weights to 2^-29: the argument as two fp32
 // numbers, a whole number R taken from it instead of the largest logit (exact, and chunks are joined by powers of
 // two), 2^y = 2^(n/16) 2^f with the sixteen powers kept in two parts and 2^f - 1, at most 1/32, from its series; its sums run in
-// fp64, and where a drafter's q is taken off it sums Z once more in the same way.
+// fp64; and where a drafter's q is taken off it sums Z once more in the same way.
 #include <algorithm>
 #include <cmath>
 
@@ -31,7 +31,7 @@ constexpr int VD_CLUSTER = 8;
 constexpr int VD_MAX_DRAFTS = 255;
 constexpr int VD_ROUND = 64;                      // steps of 128 logits that a block walks at a time
 
-struct VdPart {                                   // of one chunk of one row
+struct __align__(16) VdPart {                     // of one chunk of one row
     double sum;
     float top;
     int at;                                       // -1: no logit above -inf
@@ -217,14 +217,20 @@ __global__ void __launch_bounds__(VD_THREADS, VD_RESIDENT) verify_stats_kernel(c
 // One warp: a row's arg-max and Z relative to it.
 template <bool GREEDY>
 __device__ __forceinline__ void vd_join(const VerifyArgs& a, int row, int lane, VdBest& best, double& z) {
-    const VdPart* p = a.part + (int64_t)row * a.chunks;
-    best = VdBest{-INFINITY, -1};
-    for (int c = lane; c < a.chunks; c += 32) best = vd_better(best, VdBest{__ldcg(&p[c].top), __ldcg(&p[c].at)});
+    const float4* p = reinterpret_cast<const float4*>(a.part + (int64_t)row * a.chunks);       // sum (two words), top, at
+    const float4 none = make_float4(0.0f, 0.0f, -INFINITY, __int_as_float(-1)), own = lane < a.chunks ? __ldcg(p + lane) : none;
+    best = VdBest{own.z, __float_as_int(own.w)};
+    for (int c = lane + 32; c < a.chunks; c += 32) {
+        const float4 f = __ldcg(p + c);
+        best = vd_better(best, VdBest{f.z, __float_as_int(f.w)});
+    }
     best = vd_warp_best(best);
     z = 0.0;
     if (!GREEDY) {
-        for (int c = lane; c < a.chunks; c += 32)
-            if (__ldcg(&p[c].at) >= 0) z += __ldcg(&p[c].sum) * vd_rescale(a, __ldcg(&p[c].top), best.v);
+        for (int c = lane; c < a.chunks; c += 32) {
+            const float4 f = c == lane ? own : __ldcg(p + c);
+            if (__float_as_int(f.w) >= 0) z += __hiloint2double(__float_as_int(f.y), __float_as_int(f.x)) * vd_rescale(a, f.z, best.v);
+        }
         z = warp_sum_d(z);
     }
 }
@@ -235,7 +241,7 @@ __global__ void __launch_bounds__(VD_THREADS, VD_RESIDENT) verify_pick_kernel(co
     __shared__ bool s_keep[VD_MAX_DRAFTS + 1];
     __shared__ float s_top[VD_MAX_DRAFTS + 1];
     __shared__ int s_at[VD_MAX_DRAFTS + 1];
-    __shared__ double s_mass[3][VD_WARPS];
+    __shared__ double s_z[VD_MAX_DRAFTS + 1], s_mass[3][3][VD_WARPS];      // by pass: masses, and with a drafter's q what they lose with Z, all of p
     __shared__ int2 s_pow[16];
     __shared__ double s_step[VD_ROUND];
     cg::cluster_group cluster = cg::this_cluster();
@@ -272,6 +278,7 @@ __global__ void __launch_bounds__(VD_THREADS, VD_RESIDENT) verify_pick_kernel(co
             s_keep[j] = keep;
             s_top[j] = best.v;
             s_at[j] = best.i;
+            s_z[j] = z;
         }
     }
     __syncthreads();
@@ -285,7 +292,7 @@ __global__ void __launch_bounds__(VD_THREADS, VD_RESIDENT) verify_pick_kernel(co
         const float* q = refused && a.draft ? a.draft + row * a.ds : nullptr;
         const int without = refused && !a.draft ? a.ids[row + 1] : -1;
         const float top = s_top[n];
-        double z = 0.0;
+        double z = s_z[n];
         const VdWeights weigh = vd_weights(a, s_pow, top);
         // segment of a warp: whole steps of 128 logits
         const int steps = ((a.V + 127) / 128 + VD_CLUSTER * VD_WARPS - 1) / (VD_CLUSTER * VD_WARPS), seg = steps * 128;
@@ -333,34 +340,42 @@ __global__ void __launch_bounds__(VD_THREADS, VD_RESIDENT) verify_pick_kernel(co
             }
         };
         const int own = (rank * VD_WARPS + warp) * seg;
-        bool from_p = !refused || q;               // with a drafter's q, first Z: the mass of all of p
+        // With a drafter's q: the masses for the first kernel's Z, which is off by up to 1e-7, how they change with Z, and all of p, which is
+        // the Z they are then corrected to.  What of p is left where p and q nearly agree is summed again for the right Z.
+        bool from_p = !refused;
         double lane_from = 0.0, lane_mid = 0.0, lane_to = 0.0, total = 0.0;
         for (int pass = 0; pass < 3; ++pass) {
-            double sum = 0.0;
-            float rest = 0.0f;                     // what the weights' second parts come to, 2^-24 of the sum: in fp32
+            double sum = 0.0, whole = 0.0;
+            float rest = 0.0f, whole_rest = 0.0f, loses = 0.0f;       // rests: what the weights' second parts come to, 2^-24 of the sum
             const bool with_q = !from_p && q;
             auto add = [&](int at, const Four& f) {
                 float hi[4], lo[4];
                 weights(f, hi, lo);
-                if (with_q) {
-                    const float y[4] = {f.q.x, f.q.y, f.q.z, f.q.w};
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const double r = fma(-(double)y[k], z, (double)hi[k]);
-                        if (r > 0.0) {
-                            sum += r;
-                            rest += lo[k];
-                        }
-                    }
-                    return;
-                }
                 if (!from_p && (unsigned)(without - at) < 4u) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         if (at + k == without) hi[k] = lo[k] = 0.0f;
                 }
-                sum += ((double)hi[0] + (double)hi[1]) + ((double)hi[2] + (double)hi[3]);
-                rest += (lo[0] + lo[1]) + (lo[2] + lo[3]);
+                const double h[4] = {(double)hi[0], (double)hi[1], (double)hi[2], (double)hi[3]};
+                const double all = (h[0] + h[1]) + (h[2] + h[3]);
+                const float low = (lo[0] + lo[1]) + (lo[2] + lo[3]);
+                if (!with_q) {
+                    sum += all;
+                    rest += low;
+                    return;
+                }
+                whole += all;
+                whole_rest += low;
+                const float y[4] = {f.q.x, f.q.y, f.q.z, f.q.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const double r = fma(-(double)y[k], z, h[k]);
+                    if (r > 0.0) {
+                        sum += r;
+                        rest += lo[k];
+                        loses += y[k];
+                    }
+                }
             };
             // two steps at a time, the next two under way
             auto fetch = [&](int s, Four (&f)[2]) {
@@ -379,14 +394,27 @@ __global__ void __launch_bounds__(VD_THREADS, VD_RESIDENT) verify_pick_kernel(co
                 fetch(s + 4, u);
                 take(s + 2, v);
             }
-            sum += (double)rest;
-            sum = warp_sum_d(sum);
-            if (lane == 0) s_mass[pass][warp] = sum;
+            sum = warp_sum_d(sum + (double)rest);
+            if (with_q) {
+                whole = warp_sum_d(whole + (double)whole_rest);
+                loses = warp_sum(loses);
+            }
+            if (lane == 0) {
+                s_mass[pass][0][warp] = sum;
+                s_mass[pass][1][warp] = (double)loses;
+                s_mass[pass][2][warp] = whole;
+            }
             cluster.sync();
             // where the segments begin and end on the line of masses, the same numbers in every warp: lane k has segments 2 k and
             // 2 k + 1, [prev, mid) and [mid, upto), made to ascend whatever the sums' rounding
-            const double* of = cluster.map_shared_rank(&s_mass[pass][0], lane / 4) + 2 * (lane % 4);
-            const double m0 = of[0], m1 = of[1];
+            const double* of = cluster.map_shared_rank(&s_mass[pass][0][0], lane / 4) + 2 * (lane % 4);
+            double m0 = of[0], m1 = of[1];
+            if (with_q) {
+                const double e0 = of[2 * VD_WARPS], e1 = of[2 * VD_WARPS + 1], right = warp_sum_d(e0 + e1), more = right - z;
+                m0 = fmax(m0 - more * of[VD_WARPS], 0.0);
+                m1 = fmax(m1 - more * of[VD_WARPS + 1], 0.0);
+                z = right;
+            }
             double upto = m0 + m1;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -403,11 +431,7 @@ __global__ void __launch_bounds__(VD_THREADS, VD_RESIDENT) verify_pick_kernel(co
             lane_from = prev;
             lane_mid = mid;
             lane_to = upto;
-            if (pass == 0 && refused && q) {
-                z = total;
-                from_p = false;
-                continue;
-            }
+            if (with_q && pass == 0 && total < 1e-3 * z) continue;
             if (total > 0.0 || from_p) break;
             from_p = true;                         // max(p - q, 0) has no mass
         }
