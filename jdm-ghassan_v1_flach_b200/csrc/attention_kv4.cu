@@ -100,12 +100,7 @@ __device__ __forceinline__ float a4_exp2(float x) {
     return y;
 }
 template <int BYTES>
-__device__ __forceinline__ void a4_copy(uint32_t dst, const uint8_t* src) {
-    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
-}
-template <int BYTES>
-__device__ __forceinline__ void a4_copy(uint32_t dst, const uint8_t* src, bool there) {   // zeros where there is nothing
+__device__ __forceinline__ void a4_copy(uint32_t dst, const uint8_t* src, bool there) {   // zeros where there is nothing (src is an address all the same)
     if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
     else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(there ? BYTES : 0) : "memory");
 }
@@ -250,13 +245,14 @@ __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(c
         const int pair0 = tile * PAIRS, npairs = seq.rows * a.group;
 
         // ---- one tile of 32 keys into stage s ----
-        // K rows stand in the order in which the fragments take them, V rows as they come, the pieces of every other pair of rows swapped
-        // so that four rows one apart miss each other's banks
-        constexpr int CH = ST::ROW / 16, PER = 32 / CH;          // 16-byte pieces of a row, keys per round
-        const int lkey = lane / CH, lpiece = lane % CH * 16;
-        const uint32_t kdst = ring_at + ((lkey & 8) + 2 * (lkey & 3) + ((lkey >> 2) & 1)) * ST::ROW + lpiece;
+        // A lane brings pieces of 16 bytes of its half's keys, PER keys of the half a round.  K rows stand in the order in which the fragments take them,
+        // V rows as they come, the pieces of every other pair of rows swapped so that four rows one apart miss each other's banks.
+        constexpr int CH = ST::ROW / 16, PER = 16 / CH;
+        const int hkey = lane % 16 / CH, lkey = (lane & 16) + hkey, lpiece = lane % CH * 16;
+        const uint32_t kdst = ring_at + ((lane & 16) + 2 * (hkey & 3) + (hkey >> 2)) * ST::ROW + lpiece;
         const uint32_t vdst = ring_at + ST::V + lkey * ST::ROW + (HD == 128 ? lpiece ^ ((lkey & 2) * 16) : lpiece);
         const uint32_t sdst = ring_at + ST::KS + lane * ST::SROW;
+        auto k_round = [](int i) { return HD == 128 ? (i >> 1) * 8 + (i & 1) : 8 * i; };           // rows on, in K's order
         const int kv_row = kv * a.page;
         // Page and token in it of the tile's keys: a lane has the first key of its half (sixteen keys lie in one page), or, where pages do
         // not allow that, its own key.
@@ -278,34 +274,39 @@ __global__ void __launch_bounds__(A4_THREADS, a4_resident(NT)) attn_kv4_kernel(c
             const uint8_t* at = a.pages + (uint64_t)(there ? (uint32_t)pl.id : 0u) * a.page_bytes;
             const uint8_t* codes = at + (uint32_t)(kv_row + pl.off) * ST::ROW;
             const uint8_t* scales = at + a.k_scale + (uint32_t)(kv_row + pl.off + (halves ? lane & 15 : 0)) * ST::SROW;
-            if (halves && k + A4_KEYS <= kend && __all_sync(0xffffffffu, there)) {
-                const uint8_t* half[2];
+            if (halves) {
+                const uint8_t* p = codes + hkey * ST::ROW + lpiece;
+                if (k + A4_KEYS <= kend) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    half[h] = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(codes), 16 * h)) + (lkey * ST::ROW + lpiece);
-#pragma unroll
-                for (int i = 0; i < A4_KEYS / PER; ++i) {
-                    const uint8_t* p = half[i * PER / 16] + i * PER % 16 * ST::ROW;
-                    a4_copy<16>(kdst + so + i * PER * ST::ROW, p);
-                    a4_copy<16>(vdst + so + i * PER * ST::ROW, p + a.v_code);
+                    for (int i = 0; i < CH; ++i) {
+                        a4_copy<16>(kdst + so + k_round(i) * ST::ROW, p + i * PER * ST::ROW, there);
+                        a4_copy<16>(vdst + so + i * PER * ST::ROW, p + a.v_code + i * PER * ST::ROW, there);
+                    }
+                    a4_copy<ST::SROW>(sdst + so, scales, there);
+                    a4_copy<ST::SROW>(sdst + so + (ST::VS - ST::KS), scales + a.v_code, there);      // V's parts follow K's in the same order
+                    return;
                 }
-                a4_copy<ST::SROW>(sdst + so, scales);
-                a4_copy<ST::SROW>(sdst + so + (ST::VS - ST::KS), scales + a.v_code);       // the V parts follow the K parts in the same order
-                return;
-            }
 #pragma unroll
-            for (int i = 0; i < A4_KEYS / PER; ++i) {
-                const int key_of = i * PER + lkey, of = halves ? key_of & 16 : key_of;
-                const uint8_t* p = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(codes), of));
-                const bool ok = __shfl_sync(0xffffffffu, there, of) && k + key_of < kend;
-                p = ok ? p + (halves ? key_of & 15 : 0) * ST::ROW + lpiece : a.pages;
-                a4_copy<16>(kdst + so + i * PER * ST::ROW, p, ok);
-                a4_copy<16>(vdst + so + i * PER * ST::ROW, p + a.v_code, ok);
+                for (int i = 0; i < CH; ++i) {
+                    const bool ok = there && k + lkey + i * PER < kend;
+                    const uint8_t* from = ok ? p + i * PER * ST::ROW : a.pages;
+                    a4_copy<16>(kdst + so + k_round(i) * ST::ROW, from, ok);
+                    a4_copy<16>(vdst + so + i * PER * ST::ROW, from + a.v_code, ok);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < CH; ++i) {
+                    const int key_of = lkey + i * PER;
+                    const uint8_t* p = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(codes), key_of)) + lpiece;
+                    const bool ok = __shfl_sync(0xffffffffu, there, key_of) && k + key_of < kend;
+                    a4_copy<16>(kdst + so + k_round(i) * ST::ROW, p, ok);
+                    a4_copy<16>(vdst + so + i * PER * ST::ROW, p + a.v_code, ok);
+                }
             }
-            const bool ok = k + lane < kend && there;
-            const uint8_t* p = ok ? scales : a.pages;
-            a4_copy<ST::SROW>(sdst + so, p, ok);
-            a4_copy<ST::SROW>(sdst + so + (ST::VS - ST::KS), p + a.v_code, ok);
+            const bool ok = there && k + lane < kend;
+            const uint8_t* from = ok ? scales : a.pages;
+            a4_copy<ST::SROW>(sdst + so, from, ok);
+            a4_copy<ST::SROW>(sdst + so + (ST::VS - ST::KS), from + a.v_code, ok);
         };
         auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
 
