@@ -12,8 +12,8 @@
  *
  * Conventions are those of b200ops.h: device pointers, the library's current stream, status codes.  None of
  * these calls allocates, synchronises or keeps anything between calls, so all of them can be captured into
- * CUDA graphs (the rest of b200_rope_frequencies, which fills a table once, included); where a call needs room,
- * the caller gives it a workspace, any contents, 16-byte aligned, not shared by calls that may overlap.
+ * CUDA graphs; where a call needs room, the caller gives it a workspace, any contents, 16-byte aligned, not shared by
+ * calls that may overlap.
  * Lengths and offsets are read on the device when the call runs.
  *
  * The 4-bit pages.  `pages` holds num_pages pages of b200_kv4_page_bytes() bytes, 16-byte aligned, each of `page`
@@ -23,7 +23,7 @@
  * kind 0 (Q4_0): a scale is one fp16 d, the value d * (code - 8); kind 1 (Q4_1): an fp16 pair d, m, the value
  * d * code + m.  kind 0 holds the codes and scales of b200_quantize, bit for bit; kind 1 as well, but that its step is
  * (max - min) * fp32(1/15), not a division: its last bit may differ and with it the code of a value on the border of two.  d and m beyond
- * the range of fp16 are kept as +-65504 (every stored value is finite).  Slot s is token s % page of page s / page;
+ * the range of fp16 are kept as +-65504.  So every stored value is finite and no d is negative, which the attention counts on.  Slot s is token s % page of page s / page;
  * num_pages * page must fit in 31 bits, KV * page be at most 2^23. */
 #ifndef B200SERVE_H
 #define B200SERVE_H
@@ -69,7 +69,7 @@ int b200_rope_frequencies(double* inv_freq, int rot_dim, double theta, int scali
 /* The first rot_dim (even, <= head_dim <= 1024) elements of every head turned by pos * inv_freq, the rest copied.  rope_type as
  * in b200_rope_forward_cached: 0 pairs (2i, 2i+1), 1 pairs (i, i + rot_dim/2).  q [ntok, n_heads, head_dim] with q_stride
  * floats from token to token, k [ntok, n_kv, head_dim] likewise, outputs with strides of their own; an output may be its
- * input (then with the same stride), else they must not overlap.  q (and q_out) or k (and k_out) may be NULL.  A row with a negative
+ * input (then with the same stride) or other columns of the same rows, else they must not overlap.  q (and q_out) or k (and k_out) may be NULL.  A row with a negative
  * position is left as it was.  The angle is taken in 64 bits and reduced before cos and sin. */
 int b200_rope_forward_scaled(const float* q, const float* k, float* q_out, float* k_out, const int32_t* pos,
                              const double* inv_freq, int64_t ntok, int n_heads, int n_kv, int head_dim, int rot_dim,
@@ -94,8 +94,7 @@ int b200_kv4_fetch(const void* pages, int num_pages, int page, const int32_t* sl
  * beyond max_pages * page is cut to it; a page id outside [0, num_pages) reads as zeros.  A row before the sequence's first
  * token (more rows than tokens) is all zeros; rows of no sequence are left as they were.  fp32 accuracy: queries and
  * probabilities travel as two fp16 parts that hold 2^-24 of the largest among them (of a query's elements; of 32 tokens' weights), codes are
- * exact, sums are fp32.  hd and strides multiples of 4, q, out and pages
- * 16-byte aligned.  workspace: b200_attention_paged_kv4_workspace() bytes for the same H, KV, hd, max_rows (the batch
+ * exact, sums are fp32.  q, out and pages 16-byte aligned, strides multiples of 4.  workspace: b200_attention_paged_kv4_workspace() bytes for the same H, KV, hd, max_rows (the batch
  * and the lengths do not matter). */
 int b200_attention_paged_kv4_workspace(int H, int KV, int hd, int max_rows, size_t* bytes);
 int b200_attention_paged_kv4(const float* q, int64_t q_stride, const int32_t* row_offsets, const void* pages, int num_pages,
@@ -108,7 +107,7 @@ int b200_attention_paged_kv4(const float* q, int64_t q_stride, const int32_t* ro
  * by the row before.  p = softmax(logits / temperature) (temperature <= 0: greedy, at most 1e30); q: the row of draft_probs [rows, V] that the
  * draft was drawn from (NULL: the drafter had no choice, q(x) = 1).  Draft x is kept iff u * q(x) < p(x), u = uniforms of the
  * checking row, in [0, 1); the first refusal draws from max(p - q, 0) (q = 1 at x alone if draft_probs is NULL), and if there is none
- * the next token is drawn from the last row's p: the first index whose cumulated mass exceeds u * (all of it), u = the
+ * the next token is drawn from the p of the row behind the last draft: the first index whose cumulated mass exceeds u * (all of it), u = the
  * uniform of the sequence's last row, or from p itself where max(p - q, 0) has no mass.  Greedy: a draft is kept iff it is the arg-max
  * (the lowest index of equal ones), the next token is the arg-max.  NaN logits count as -inf; several +inf share the mass; a row
  * without any logit above -inf keeps no draft and draws -1, as does an id outside the vocabulary keep nothing.

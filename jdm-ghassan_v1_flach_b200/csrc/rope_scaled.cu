@@ -199,7 +199,11 @@ int b200_rope_forward_scaled(const float* q, const float* k, float* q_out, float
     B200_REQUIRE((!q || (q_stride >= qn && q_out_stride >= qn)) && (!k || (k_stride >= kn && k_out_stride >= kn)),
                  "%s: a stride is shorter than its row", who);
     auto apart = [&](const float* x, int64_t xs, const float* y, int64_t ys, int64_t n) {
-        return (x == y && xs == ys) || x + (ntok - 1) * xs + n <= y || y + (ntok - 1) * ys + n <= x;
+        if (x + (ntok - 1) * xs + n <= y || y + (ntok - 1) * ys + n <= x) return true;
+        if (xs != ys) return false;
+        // the same rows: the same columns, or others of each row
+        const int64_t off = ((int64_t)(reinterpret_cast<intptr_t>(y) - reinterpret_cast<intptr_t>(x)) / (int64_t)sizeof(float) % xs + xs) % xs;
+        return x == y || (off >= n && xs - off >= n);
     };
     B200_REQUIRE((!q || apart(q, q_stride, q_out, q_out_stride, qn)) && (!k || apart(k, k_stride, k_out, k_out_stride, kn)),
                  "%s: an output overlaps its input without being it", who);

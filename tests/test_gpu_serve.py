@@ -132,6 +132,17 @@ def test_rope(rope_type, n, H, KV, hd, rot, pad):
     assert torch.equal(alone[live].reshape(-1, KV * hd), ko[live])
 
 
+def test_rope_into_other_columns_of_the_same_rows():
+    r = np.random.default_rng(6)
+    x = r.standard_normal((5, 400)).astype(np.float32)
+    buf, f, p = dev(x), torch.tensor(so.frequencies(16, 1e4, 0, 1.0, 1, 1.0, 2.0), device="cuda"), i32([3, 1, 4, 1, 5])
+    ops.rope_forward_scaled(buf, None, buf[:, 130:], None, p, f, 5, 2, 0, 64, 16, 1, 400, 0, 400, 0, 1.0)
+    got = host(buf)
+    want = so.rope(x[:, :128].reshape(5, 2, 64), [3, 1, 4, 1, 5], host(f), 16, 1, 1.0).reshape(5, 128)
+    assert np.abs(got[:, 130:258] - want).max() <= 4 * ROPE_TOL * np.abs(x).max()
+    assert np.array_equal(got[:, :130], x[:, :130]) and np.array_equal(got[:, 258:], x[:, 258:])
+
+
 def test_rope_agrees_with_the_cached_form():
     """Unscaled, whole head: the framework's own rotation up to its fp32 angle (2^-24 of the angle, here at most 500)."""
     r = np.random.default_rng(5)
@@ -398,6 +409,22 @@ def test_attention_far_into_a_large_pool():
     ops.kv4_fetch(pages, len(pages), page, i32(slots), 2, a, b, KV * hd, KV * hd, KV, hd, 1)
     assert np.array_equal(host(a), so.values(*so.quantize(x, 1), 1).astype(np.float32))
     assert np.array_equal(host(b), so.values(*so.quantize(-x, 1), 1).astype(np.float32))
+
+
+@pytest.mark.parametrize("kind", [0, 1])
+def test_attention_of_a_long_context(kind):
+    """70 001 tokens of one sequence beside short ones: hundreds of pieces of one item."""
+    r = np.random.default_rng(62)
+    H, KV, hd, page, lens, rows = 4, 1, 128, 64, [70001, 3, 500], [2, 1, 1]
+    cache, table, kv = make_cache(r, lens, page, KV, hd, kind)
+    q, offs = r.standard_normal((4, H, hd)).astype(np.float32), np.array([0, 2, 3, 4])
+    out = empty((4, H, hd))
+    call_attention(dev(q), H * hd, i32(offs), dev(cache.bytes), cache.num_pages, i32(table), i32(lens), out, H * hd, 2, page, H, KV, hd, kind, 0.088, 0)
+    want = np.concatenate([so.attention(q, offs[b], rows[b], lens[b], *kv[b], np.float32(0.088), 0) for b in range(3)])
+    got = host(out).astype(np.float64)
+    assert np.abs(got - want).max() <= attention_bound(q, kv, 0.088)
+    # the long one alone, whose values average out to a hundredth: in its own size.  A weight is off by 2^-21 at most, with either sign
+    assert np.linalg.norm(got[:2] - want[:2]) <= 2.0 ** -19 * np.linalg.norm(want[:2])
 
 
 def test_attention_with_a_window_beyond_every_length():

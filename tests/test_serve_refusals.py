@@ -44,7 +44,7 @@ ROPE = dict(q=P, k=2 * P, q_out=P, k_out=2 * P, pos=P, freq=P, n=4, H=4, KV=2, h
 
 
 @pytest.mark.parametrize("change", [dict(pos=None), dict(freq=None), dict(q=None), dict(k_out=None), dict(rot=0), dict(rot=31), dict(rot=66),
-                                    dict(hd=1026), dict(type=2), dict(H=0), dict(KV=0), dict(qs=255), dict(kos=127), dict(qos=512),
+                                    dict(hd=1026), dict(type=2), dict(H=0), dict(KV=0), dict(qs=255), dict(kos=127), dict(qos=512), dict(q_out=P + 4 * 200), dict(qs=400, qos=400, q_out=P + 4 * 200),
                                     dict(q_out=P + 64), dict(k_out=2 * P + 4, k=2 * P), dict(q=None, q_out=None, k=None, k_out=None),
                                     dict(type=0, hd=63, qs=256, rot=32)])
 def test_rope(change):
