@@ -16,15 +16,16 @@
 //   O^T [16 dims, 4 pairs x 2 parts] = V^T [16 dims, 16 keys] . (p d)^T, the weights' fragments turned by movmatrix
 // (pair: a query row and one of the heads that share the KV head).
 //
-// What bounds it: for single tokens the cache, 2 KV (hd/2 + 4 hd/32) bytes a token once (kind 1), with about 600 instructions of a
-// warp per 32 keys behind it - two thirds of what an SM can issue in the time the bytes take; for many rows the instructions.
+// What bounds it: for single tokens the cache, 2 KV (hd/2 + 4 hd/32) bytes a token once (kind 1), with about 730 instructions of a
+// warp per 32 keys behind it, which is what the time goes to (57 % of the issue slots; 64 sequences of 256 to 8192 tokens, 32 / 8 heads of
+// 128: 55 us, the bytes alone 29); for many rows the instructions more still.
 //
 // The split.  The lengths are on the device, so the grid is fixed and every warp takes an equal share of all (sequence, KV head, tile of
 // 4 or 8 pairs, 32 keys) units laid end to end, with what an item's set-up costs counted in, found from a prefix sum over the batch that
 // every block makes by itself.  What a share cuts off an item's ends goes to the workspace and is joined by a second, small kernel.
-// (Shares of whole blocks, their warps joined in shared memory: 74 us where this takes 64.  Warps of a block on different pairs of the
+// (Shares of whole blocks, their warps joined in shared memory: 74 us where this took 64 then, and takes 55 now.  Warps of a block on different pairs of the
 // same keys: idle ones where the pairs are no multiple, 149 us on the drafts below.)  Keys come through a ring of each warp's own in
-// shared memory that cp.async fills one or two tiles ahead.
+// shared memory that cp.async fills a tile ahead.
 #include <algorithm>
 #include <type_traits>
 
