@@ -52,9 +52,41 @@ __device__ __forceinline__ float kc_min(float a, float b) {
     asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-// The nearest whole number to v >= 0, halves up, as the low bits: floor(v + 1/2), both steps rounded down, which never passes a whole
-// number that the exact sum has not reached.
-__device__ __forceinline__ int kc_nearest(float v) { return __float_as_int(__fadd_rd(__fadd_rd(v, 0.5f), 8388608.0f)); }
+// Two sums, rounded down.
+__device__ __forceinline__ f32x2 kc_add_down(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rm.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// floor(y + shift), 0 .. 15, of four numbers as nibbles, lowest first, with anything above the low 24 bits: both steps are rounded down,
+// which never passes a whole number that the exact sum has not reached, and leave the floor in the low bits of a number of
+// exponent 23, the rest of which only reaches bits 24 and up.
+__device__ __forceinline__ uint32_t kc_codes(const float2 (&y)[2], float shift) {
+    uint32_t code = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float2 f = each(kc_add_down(kc_add_down(two(y[i].x, y[i].y), two(shift, shift)), two(8388608.0f, 8388608.0f)));
+        code += ((uint32_t)__float_as_int(f.x) << (8 * i)) + ((uint32_t)__float_as_int(f.y) << (8 * i + 4));
+    }
+    return code;
+}
+// One of NB values that eight lanes have each, joined over them: lane g has the one of block g % NB.  Half of the values go
+// to a neighbour at each of the first steps, and half as many are left.
+template <int NB, typename Join>
+__device__ __forceinline__ float kc_join(const float (&x)[NB], int g, Join join) {
+    float r;
+    if (NB == 4) {
+        const bool far = g & 2, odd = g & 1;
+        const float a = join(far ? x[2 % NB] : x[0], __shfl_xor_sync(0xffffffffu, far ? x[0] : x[2 % NB], 2));
+        const float b = join(far ? x[3 % NB] : x[1], __shfl_xor_sync(0xffffffffu, far ? x[1] : x[3 % NB], 2));
+        r = join(odd ? b : a, __shfl_xor_sync(0xffffffffu, odd ? a : b, 1));
+    } else {
+        const bool odd = g & 1;
+        r = join(odd ? x[1] : x[0], __shfl_xor_sync(0xffffffffu, odd ? x[0] : x[1], 1));
+        r = join(r, __shfl_xor_sync(0xffffffffu, r, 2));
+    }
+    return join(r, __shfl_xor_sync(0xffffffffu, r, 4));
+}
 
 // A row of a head: its token, its head, and where its codes and scales stand in the pages (K's or V's); slot < 0: in none.
 template <int HD, int KIND>
@@ -106,21 +138,9 @@ __global__ void __launch_bounds__(KC_THREADS) kv4_store_kernel(const __grid_cons
             hi[b] = kc_max(kc_max(fabsf(x[b][0]), fabsf(x[b][1])), kc_max(fabsf(x[b][2]), fabsf(x[b][3])));
         }
     }
-#pragma unroll
-    for (int s = 1; s < 8; s <<= 1)
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            hi[b] = kc_max(hi[b], __shfl_xor_sync(0xffffffffu, hi[b], s));
-            if (KIND == 1) lo[b] = kc_min(lo[b], __shfl_xor_sync(0xffffffffu, lo[b], s));
-        }
     // each lane makes one block's scale and inverse, and has the others' from its neighbours
-    float my_hi = hi[0], my_lo = KIND == 1 ? lo[0] : 0.0f;
-#pragma unroll
-    for (int b = 1; b < NB; ++b)
-        if (g % NB == b) {
-            my_hi = hi[b];
-            my_lo = KIND == 1 ? lo[b] : 0.0f;
-        }
+    const float my_hi = kc_join(hi, g, [](float u, float w) { return kc_max(u, w); });
+    const float my_lo = KIND == 1 ? kc_join(lo, g, [](float u, float w) { return kc_min(u, w); }) : 0.0f;
     const float d = KIND == 1 ? __fmul_rn(__fsub_rn(my_hi, my_lo), 1.0f / 15.0f) : __fmul_rn(my_hi, 0.125f);
     const bool sound = my_hi < INFINITY && my_lo > -INFINITY;
     const float my_inv = !sound ? -1.0f : d > 0.0f ? __frcp_rn(d) : 0.0f;      // -1: the block is to be zero
@@ -128,27 +148,30 @@ __global__ void __launch_bounds__(KC_THREADS) kv4_store_kernel(const __grid_cons
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         const float inv = __shfl_sync(0xffffffffu, my_inv, b, 8);
-        uint32_t code = 0;
-        if (inv >= 0.0f && inv < INFINITY) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (KIND == 1) {
-                    // at most 15 of them; above its low bits a number's exponent only reaches bits 24 and up.  hi - lo = inf: inv = 0
-                    const float y = __fmul_rn(__fsub_rn(x[b][i], lo[b]), inv);
-                    code += (uint32_t)kc_nearest(y == y ? y : 0.0f) << (4 * i);
-                } else {
-                    const float y = __fmul_rn(x[b][i], inv);
-                    const int n = kc_nearest(fabsf(y)) - 0x4B000000;              // 0 .. 8
-                    code += (uint32_t)(y < 0.0f ? 8 - n : min(8 + n, 15)) << (4 * i);
-                }
+        const float least = KIND == 1 ? __shfl_sync(0xffffffffu, my_lo, b, 8) : 0.0f;
+        uint32_t code = KIND == 0 ? 0x8888u : 0u;            // of zeros, of equal ones, of a range that is no fp32 number, and unsound
+        if (inv > 0.0f && inv < INFINITY) {
+            const f32x2 by = two(inv, inv);
+            float2 y[2];
+            if (KIND == 1) {                                 // at most 15 of them
+                y[0] = each(mul2(add2(two(x[b][0], x[b][1]), two(-least, -least)), by));
+                y[1] = each(mul2(add2(two(x[b][2], x[b][3]), two(-least, -least)), by));
+                code = kc_codes(y, 0.5f);
+            } else {
+                // 8 and the nearest, halves away from zero, 16 as 15: floor(y + 8.5) but for a half below zero, which one bit further from
+                // zero is none
+                y[0] = each(mul2(two(x[b][0], x[b][1]), by));
+                y[1] = each(mul2(two(x[b][2], x[b][3]), by));
+                auto further = [](float v) { return fminf(__int_as_float(__float_as_int(v) + (int)((uint32_t)__float_as_int(v) >> 31)), 7.0f); };
+                y[0] = make_float2(further(y[0].x), further(y[0].y));
+                y[1] = make_float2(further(y[1].x), further(y[1].y));
+                code = kc_codes(y, 8.5f);
             }
-        } else if (KIND == 0) {
-            code = 0x8888u;
         }
         if (inv == INFINITY) {                               // a block of denormals: all that is not its zero (or minimum) is as far as codes go
             code = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) code |= (KIND == 1 ? (x[b][i] > lo[b] ? 15u : 0u) : x[b][i] > 0.0f ? 15u : x[b][i] < 0.0f ? 0u : 8u) << (4 * i);
+            for (int i = 0; i < 4; ++i) code |= (KIND == 1 ? (x[b][i] > least ? 15u : 0u) : x[b][i] > 0.0f ? 15u : x[b][i] < 0.0f ? 0u : 8u) << (4 * i);
         }
         word[b] = code & 0xFFFFu;
     }
