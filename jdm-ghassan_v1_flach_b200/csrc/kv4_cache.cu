@@ -6,10 +6,13 @@
 // value, because an infinite one would make a NaN of every code 0, and of every masked probability in the attention over these
 // pages.
 //
-// What bounds both: the fp32 rows (8 KV hd bytes a token), a quarter of that again for the pages' lines, with about 70 and 25
-// instructions per 16 bytes of row.  Eight lanes share a token's row of one head: lane g has the four elements 4 g .. 4 g + 3 of each block
+// What bounds both: the fp32 rows (8 KV hd bytes a token), a sixth of that again for the pages.  16 384 rows of 8 x 128, kind 0: store 27 us,
+// 5.7 TB/s, with 64 instructions a lane per 16 bytes of row behind it; fetch 26, 134 MB to write, with 48.
+// Eight lanes share a token's row of one head: lane g has the four elements 4 g .. 4 g + 3 of each block
 // of 32, which is one 16-bit word per block, and those words lie side by side.  So a warp reads and writes whole lines of the row
-// and eight bytes a lane of the codes, and a block's statistics take three shuffles.
+// and eight bytes a lane of the codes, and the statistics of four blocks take four shuffles.
+#include <type_traits>
+
 #include "serve.cuh"
 
 namespace b200 {
@@ -106,84 +109,94 @@ struct KcItem {
     }
 };
 
-// blockIdx.y: 0 K, 1 V
-template <int HD, int KIND, bool WIDE>
+// SIDES 1: K's rows or V's, by blockIdx.y; 2: a thread has its part of both, with both rows' loads under way.
+template <int HD, int KIND, bool WIDE, int SIDES>
 __global__ void __launch_bounds__(KC_THREADS) kv4_store_kernel(const __grid_constant__ Kv4Rows a) {
     constexpr int NB = HD / 32;
-    const bool v = blockIdx.y != 0;
     const int g = threadIdx.x & 7;
     short_begin();
-    const KcItem<HD, KIND> it(a, (int64_t)blockIdx.x * KC_ITEMS + (threadIdx.x >> 3), v);
-    const float* src = (v ? a.v_in + it.row * a.vs : a.k_in + it.row * a.ks) + (int64_t)it.head * HD + 4 * g;
-    float x[NB][4];
+    const KcItem<HD, KIND> it(a, (int64_t)blockIdx.x * KC_ITEMS + (threadIdx.x >> 3), false);
+    float rows[SIDES][NB][4];
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        x[b][0] = x[b][1] = x[b][2] = x[b][3] = 0.0f;
-        if (it.row < 0) continue;
-        if (WIDE) {
-            const float4 f = *reinterpret_cast<const float4*>(src + 32 * b);
-            x[b][0] = f.x; x[b][1] = f.y; x[b][2] = f.z; x[b][3] = f.w;
-        } else {
+    for (int side = 0; side < SIDES; ++side) {
+        const bool v = SIDES == 2 ? side == 1 : blockIdx.y != 0;
+        const float* src = (v ? a.v_in + it.row * a.vs : a.k_in + it.row * a.ks) + (int64_t)it.head * HD + 4 * g;
+        float(&x)[NB][4] = rows[side];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[b][i] = src[32 * b + i];
-        }
-    }
-    float lo[NB], hi[NB];                                    // kind 0: hi of the magnitudes
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        if (KIND == 1) {
-            lo[b] = kc_min(kc_min(x[b][0], x[b][1]), kc_min(x[b][2], x[b][3]));
-            hi[b] = kc_max(kc_max(x[b][0], x[b][1]), kc_max(x[b][2], x[b][3]));
-        } else {
-            hi[b] = kc_max(kc_max(fabsf(x[b][0]), fabsf(x[b][1])), kc_max(fabsf(x[b][2]), fabsf(x[b][3])));
-        }
-    }
-    // each lane makes one block's scale and inverse, and has the others' from its neighbours
-    const float my_hi = kc_join(hi, g, [](float u, float w) { return kc_max(u, w); });
-    const float my_lo = KIND == 1 ? kc_join(lo, g, [](float u, float w) { return kc_min(u, w); }) : 0.0f;
-    const float d = KIND == 1 ? __fmul_rn(__fsub_rn(my_hi, my_lo), 1.0f / 15.0f) : __fmul_rn(my_hi, 0.125f);
-    const bool sound = my_hi < INFINITY && my_lo > -INFINITY;
-    const float my_inv = !sound ? -1.0f : d > 0.0f ? __frcp_rn(d) : 0.0f;      // -1: the block is to be zero
-    uint32_t word[NB];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        const float inv = __shfl_sync(0xffffffffu, my_inv, b, 8);
-        const float least = KIND == 1 ? __shfl_sync(0xffffffffu, my_lo, b, 8) : 0.0f;
-        uint32_t code = KIND == 0 ? 0x8888u : 0u;            // of zeros, of equal ones, of a range that is no fp32 number, and unsound
-        if (inv > 0.0f && inv < INFINITY) {
-            const f32x2 by = two(inv, inv);
-            float2 y[2];
-            if (KIND == 1) {                                 // at most 15 of them
-                y[0] = each(mul2(add2(two(x[b][0], x[b][1]), two(-least, -least)), by));
-                y[1] = each(mul2(add2(two(x[b][2], x[b][3]), two(-least, -least)), by));
-                code = kc_codes(y, 0.5f);
+        for (int b = 0; b < NB; ++b) {
+            x[b][0] = x[b][1] = x[b][2] = x[b][3] = 0.0f;
+            if (it.row < 0) continue;
+            if (WIDE) {
+                const float4 f = *reinterpret_cast<const float4*>(src + 32 * b);
+                x[b][0] = f.x; x[b][1] = f.y; x[b][2] = f.z; x[b][3] = f.w;
             } else {
-                // 8 and the nearest, halves away from zero, 16 as 15: floor(y + 8.5) but for a half below zero, which one bit further from
-                // zero is none
-                y[0] = each(mul2(two(x[b][0], x[b][1]), by));
-                y[1] = each(mul2(two(x[b][2], x[b][3]), by));
-                auto further = [](float v) { return fminf(__int_as_float(__float_as_int(v) + (int)((uint32_t)__float_as_int(v) >> 31)), 7.0f); };
-                y[0] = make_float2(further(y[0].x), further(y[0].y));
-                y[1] = make_float2(further(y[1].x), further(y[1].y));
-                code = kc_codes(y, 8.5f);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[b][i] = src[32 * b + i];
             }
         }
-        if (inv == INFINITY) {                               // a block of denormals: all that is not its zero (or minimum) is as far as codes go
-            code = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) code |= (KIND == 1 ? (x[b][i] > least ? 15u : 0u) : x[b][i] > 0.0f ? 15u : x[b][i] < 0.0f ? 0u : 8u) << (4 * i);
-        }
-        word[b] = code & 0xFFFFu;
     }
-    if (it.slot < 0) return;
-    uint8_t* codes = a.pages + it.codes + g * (2 * NB);
-    if (NB == 4) *reinterpret_cast<uint2*>(codes) = make_uint2(word[0] | (word[1] << 16), word[NB > 2 ? 2 : 0] | (word[NB > 2 ? 3 : 0] << 16));
-    else *reinterpret_cast<uint32_t*>(codes) = word[0] | (word[1] << 16);
-    if (g < NB) {
-        uint8_t* scale = a.pages + it.scales + g * (KIND == 1 ? 4 : 2);
-        const float m = sound ? my_lo : 0.0f;
-        if (KIND == 1) *reinterpret_cast<uint32_t*>(scale) = sound ? kc_half(d) | (kc_half(m) << 16) : 0u;
-        else *reinterpret_cast<uint16_t*>(scale) = sound ? (uint16_t)kc_half(d) : (uint16_t)0;
+#pragma unroll
+    for (int side = 0; side < SIDES; ++side) {
+        const bool v = SIDES == 2 ? side == 1 : blockIdx.y != 0;
+        float(&x)[NB][4] = rows[side];
+        float lo[NB], hi[NB];                                    // kind 0: hi of the magnitudes
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            if (KIND == 1) {
+                lo[b] = kc_min(kc_min(x[b][0], x[b][1]), kc_min(x[b][2], x[b][3]));
+                hi[b] = kc_max(kc_max(x[b][0], x[b][1]), kc_max(x[b][2], x[b][3]));
+            } else {
+                hi[b] = kc_max(kc_max(fabsf(x[b][0]), fabsf(x[b][1])), kc_max(fabsf(x[b][2]), fabsf(x[b][3])));
+            }
+        }
+        // each lane makes one block's scale and inverse, and has the others' from its neighbours
+        const float my_hi = kc_join(hi, g, [](float u, float w) { return kc_max(u, w); });
+        const float my_lo = KIND == 1 ? kc_join(lo, g, [](float u, float w) { return kc_min(u, w); }) : 0.0f;
+        const float d = KIND == 1 ? __fmul_rn(__fsub_rn(my_hi, my_lo), 1.0f / 15.0f) : __fmul_rn(my_hi, 0.125f);
+        const bool sound = my_hi < INFINITY && my_lo > -INFINITY;
+        const float my_inv = !sound ? -1.0f : d > 0.0f ? __frcp_rn(d) : 0.0f;      // -1: the block is to be zero
+        uint32_t word[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const float inv = __shfl_sync(0xffffffffu, my_inv, b, 8);
+            const float least = KIND == 1 ? __shfl_sync(0xffffffffu, my_lo, b, 8) : 0.0f;
+            uint32_t code = KIND == 0 ? 0x8888u : 0u;            // of zeros, of equal ones, of a range that is no fp32 number, and unsound
+            if (inv > 0.0f && inv < INFINITY) {
+                const f32x2 by = two(inv, inv);
+                float2 y[2];
+                if (KIND == 1) {                                 // at most 15 of them
+                    y[0] = each(mul2(add2(two(x[b][0], x[b][1]), two(-least, -least)), by));
+                    y[1] = each(mul2(add2(two(x[b][2], x[b][3]), two(-least, -least)), by));
+                    code = kc_codes(y, 0.5f);
+                } else {
+                    // 8 and the nearest, halves away from zero, 16 as 15: floor(y + 8.5) but for a half below zero, which one bit further from
+                    // zero is none
+                    y[0] = each(mul2(two(x[b][0], x[b][1]), by));
+                    y[1] = each(mul2(two(x[b][2], x[b][3]), by));
+                    auto further = [](float v) { return fminf(__int_as_float(__float_as_int(v) + (int)((uint32_t)__float_as_int(v) >> 31)), 7.0f); };
+                    y[0] = make_float2(further(y[0].x), further(y[0].y));
+                    y[1] = make_float2(further(y[1].x), further(y[1].y));
+                    code = kc_codes(y, 8.5f);
+                }
+            }
+            if (inv == INFINITY) {                               // a block of denormals: all that is not its zero (or minimum) is as far as codes go
+                code = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) code |= (KIND == 1 ? (x[b][i] > least ? 15u : 0u) : x[b][i] > 0.0f ? 15u : x[b][i] < 0.0f ? 0u : 8u) << (4 * i);
+            }
+            word[b] = code & 0xFFFFu;
+        }
+        if (it.slot < 0) continue;
+        const int64_t side_at = v ? a.part.v_code : 0;      // V's parts follow as K's do
+        uint8_t* codes = a.pages + side_at + it.codes + g * (2 * NB);
+        if (NB == 4) *reinterpret_cast<uint2*>(codes) = make_uint2(word[0] | (word[1] << 16), word[NB > 2 ? 2 : 0] | (word[NB > 2 ? 3 : 0] << 16));
+        else *reinterpret_cast<uint32_t*>(codes) = word[0] | (word[1] << 16);
+        if (g < NB) {
+            uint8_t* scale = a.pages + side_at + it.scales + g * (KIND == 1 ? 4 : 2);
+            const float m = sound ? my_lo : 0.0f;
+            if (KIND == 1) *reinterpret_cast<uint32_t*>(scale) = sound ? kc_half(d) | (kc_half(m) << 16) : 0u;
+            else *reinterpret_cast<uint16_t*>(scale) = sound ? (uint16_t)kc_half(d) : (uint16_t)0;
+        }
     }
 }
 
@@ -267,11 +280,21 @@ int b200_kv4_store(const float* k, const float* v, int64_t k_stride, int64_t v_s
     kc_geometry(a, pages, num_pages, page, KV, hd, kind);
     a.k_in = k; a.v_in = v; a.ks = k_stride; a.vs = v_stride; a.slots = slots; a.n = n;
     const bool wide = aligned16(k) && aligned16(v) && k_stride % 4 == 0 && v_stride % 4 == 0;
-    const dim3 grid((unsigned)ceil_div64(n * KV, KC_ITEMS), 2), block(KC_THREADS);
-    auto kern = hd == 64 ? (kind == 1 ? (wide ? kv4_store_kernel<64, 1, true> : kv4_store_kernel<64, 1, false>)
-                                      : (wide ? kv4_store_kernel<64, 0, true> : kv4_store_kernel<64, 0, false>))
-                         : (kind == 1 ? (wide ? kv4_store_kernel<128, 1, true> : kv4_store_kernel<128, 1, false>)
-                                      : (wide ? kv4_store_kernel<128, 0, true> : kv4_store_kernel<128, 0, false>));
+    // A thread with both sides finds one address for them and has twice the loads under way, in half as many blocks: better as soon as
+    // these are one an SM (8 x 128, kind 0: 512 rows 4.2 -> 3.2 us, 4096 10.4 -> 8.3, 16 384 30.3 -> 26.8; kind 1 of 4 x 64: 1024 rows 4.2 -> 2.3;
+    // one case the other way, 1024 rows of 8 x 128, kind 1, 4.6 -> 5.2).  Below, the longer thread is what is waited for (256 rows 2.4 -> 2.5).
+    const dim3 block(KC_THREADS);
+    const unsigned blocks = (unsigned)ceil_div64(n * KV, KC_ITEMS);
+    const bool both = blocks > (unsigned)num_sms();
+    const dim3 grid(blocks, both ? 1 : 2);
+    auto pick = [&](auto hd_, auto kind_) {
+        constexpr int HD = decltype(hd_)::value, KIND = decltype(kind_)::value;
+        return wide ? (both ? kv4_store_kernel<HD, KIND, true, 2> : kv4_store_kernel<HD, KIND, true, 1>)
+                    : (both ? kv4_store_kernel<HD, KIND, false, 2> : kv4_store_kernel<HD, KIND, false, 1>);
+    };
+    using std::integral_constant;
+    auto kern = hd == 64 ? (kind == 1 ? pick(integral_constant<int, 64>(), integral_constant<int, 1>()) : pick(integral_constant<int, 64>(), integral_constant<int, 0>()))
+                         : (kind == 1 ? pick(integral_constant<int, 128>(), integral_constant<int, 1>()) : pick(integral_constant<int, 128>(), integral_constant<int, 0>()));
     return launch_serve("kv4_store_kernel", kern, grid, block, 0, 1, short_grid(grid), a);
 }
 

@@ -202,6 +202,28 @@ def test_store_and_fetch(kind, n, page, KV, hd, pad):
         assert both or torch.isnan(gk).all()
 
 
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("n,page,KV,hd,pad", [(4801, 16, 1, 64, 0), (1603, 64, 3, 64, 1), (811, 32, 5, 128, 4), (2051, 128, 2, 128, 3)])
+def test_store_of_many_rows(kind, n, page, KV, hd, pad):
+    """Enough rows that a thread has K and V of one; half of them have values halfway between codes."""
+    r = np.random.default_rng(n)
+    num_pages = n // page + 2
+    k, v = tricky_rows(r, n, KV, hd), tricky_rows(r, n, KV, hd)[::-1].copy()
+    k[1::2] = r.integers(-16, 17, k[1::2].shape) / 2.0 * 2.0 ** r.integers(-20, 20, (len(k[1::2]), KV, 1))
+    v[1::2] = r.integers(0, 31, v[1::2].shape) / 2.0
+    slots = r.permutation(num_pages * page)[:n]
+    slots[n // 2], slots[n - 2] = -7, num_pages * page + 5
+    cache = so.Cache(num_pages, page, KV, hd, kind, fill=0x5A)
+    pages = dev(cache.bytes)
+    cache.store(k, v, slots)
+    row = KV * hd + pad
+    src = [torch.full((n, row), 7.0, device="cuda") for _ in range(2)]
+    for s, x in zip(src, (k, v)):
+        s[:, :KV * hd] = dev(x.reshape(n, -1))
+    ops.kv4_store(src[0], src[1], row, row, i32(slots), n, pages, num_pages, page, KV, hd, kind)
+    assert np.array_equal(host(pages), cache.bytes)
+
+
 # ---- attention -----------------------------------------------------------------------------------
 def make_cache(r, lens, page, KV, hd, kind, scale=1.0):
     """A cache in host memory with rows of about unit size in the pages of len(lens) sequences, junk everywhere else."""
