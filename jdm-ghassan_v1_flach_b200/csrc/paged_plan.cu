@@ -49,14 +49,20 @@ __global__ void __launch_bounds__(PP_THREADS) paged_plan_kernel(const __grid_con
     __shared__ int s_row[PP_BATCH + 1], s_take[PP_BATCH + 1], s_back[PP_BATCH], s_ctx[PP_BATCH], s_held[PP_BATCH];
     __shared__ long long s_part[PP_THREADS / 32][3];
     __shared__ int s_most[2], s_refused;
+    __shared__ uint32_t s_ring[2];                 // where the ring starts and ends
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     short_begin();
     const long long head = a.at[0], tail = a.at[1];
     const bool sound = head >= 0 && tail >= head && tail - head <= (long long)a.ring_size;
     const long long avail = sound ? tail - head : 0;
-    const uint32_t ring_head = sound ? (uint32_t)(head % a.ring_size) : 0, ring_tail = sound ? (uint32_t)(tail % a.ring_size) : 0;
-    if (tid < 2) s_most[tid] = 0;
-    if (tid == 2) s_refused = 0;
+    const int warps = (a.batch + 32 * PP_EACH - 1) / (32 * PP_EACH);        // that have requests
+    if (warp == PP_THREADS / 32 - 1) {             // the one that has them last; a quotient of 64 bits is a hundred instructions
+        if (lane < 2) {
+            s_ring[lane] = sound ? (uint32_t)((lane ? tail : head) % a.ring_size) : 0;
+            s_most[lane] = 0;
+        }
+        if (lane == 2) s_refused = 0;
+    }
     int ctx[PP_EACH], fresh[PP_EACH], held[PP_EACH];
     long long rows[PP_EACH], take[PP_EACH], back[PP_EACH], sum[3] = {0, 0, 0};
 #pragma unroll
@@ -69,29 +75,31 @@ __global__ void __launch_bounds__(PP_THREADS) paged_plan_kernel(const __grid_con
     }
 #pragma unroll
     for (int i = 0; i < PP_EACH; ++i) {
-        const long long want = (long long)ctx[i] + fresh[i];
-        const bool fits = fresh[i] > 0 && ctx[i] >= 0 && held[i] >= 0 && held[i] <= a.max_pages && want <= (long long)a.max_pages * a.page;
+        const uint32_t want = (uint32_t)ctx[i] + (uint32_t)fresh[i];        // of two numbers below 2^31
+        const bool fits = fresh[i] > 0 && ctx[i] >= 0 && held[i] >= 0 && held[i] <= a.max_pages && want <= (uint32_t)(a.max_pages * a.page);
         rows[i] = fits ? fresh[i] : 0;
-        take[i] = fits ? max(0ll, (want + a.page - 1) / a.page - held[i]) : 0;
+        const uint32_t full = a.by_page.div(fits ? want : 0u), pages = full + (want > full * a.page);
+        take[i] = fits ? max(0, (int)pages - held[i]) : 0;
         back[i] = fresh[i] < 0 ? min(max(held[i], 0), a.max_pages) : 0;
         sum[0] += rows[i];
         sum[1] += take[i];
         sum[2] += back[i];
     }
-    long long before[3];
+    long long before[3] = {0, 0, 0};
+    if (warp < warps) {
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
-        long long v = sum[k];
+        for (int k = 0; k < 3; ++k) {
+            long long v = sum[k];
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long u = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= o) v += u;
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long u = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v += u;
+            }
+            before[k] = v - sum[k];
+            if (lane == 31) s_part[warp][k] = v;
         }
-        before[k] = v - sum[k];
-        if (lane == 31) s_part[warp][k] = v;
     }
     __syncthreads();
-    const int warps = (a.batch + 32 * PP_EACH - 1) / (32 * PP_EACH);        // that have requests
     long long all_back = 0;
     for (int w = 0; w < warps; ++w) {
         if (w < warp)
@@ -118,13 +126,15 @@ __global__ void __launch_bounds__(PP_THREADS) paged_plan_kernel(const __grid_con
         }
         refused += fresh[i] > 0 && !ok[i];
     }
-    most_rows = __reduce_max_sync(0xffffffffu, most_rows);
-    most_take = __reduce_max_sync(0xffffffffu, most_take);
-    refused = __reduce_add_sync(0xffffffffu, refused);
-    if (lane == 0) {
-        atomicMax(&s_most[0], most_rows);
-        atomicMax(&s_most[1], most_take);
-        if (refused) atomicAdd(&s_refused, refused);
+    if (warp < warps) {
+        most_rows = __reduce_max_sync(0xffffffffu, most_rows);
+        most_take = __reduce_max_sync(0xffffffffu, most_take);
+        refused = __reduce_add_sync(0xffffffffu, refused);
+        if (lane == 0) {
+            atomicMax(&s_most[0], most_rows);
+            atomicMax(&s_most[1], most_take);
+            if (refused) atomicAdd(&s_refused, refused);
+        }
     }
     __syncthreads();
     const int all_rows = s_most[0], all_take = s_most[1];
@@ -167,6 +177,7 @@ __global__ void __launch_bounds__(PP_THREADS) paged_plan_kernel(const __grid_con
         }
     }
     if (!a.expand) return;
+    const uint32_t ring_head = s_ring[0], ring_tail = s_ring[1];
     auto ring_index = [&](uint32_t from, uint32_t j) {      // both below the ring's size
         const uint32_t i = from + j;
         return i >= a.ring_size ? i - a.ring_size : i;
